@@ -31,6 +31,8 @@ extern "C" {
 #define B200_ELIMIT (-6)      /* problem larger than a fixed built-in limit       */
 
 #define B200_DTYPE_F16 0
+#define B200_DTYPE_BF16 1    /* the operators from b200_rotate on */
+#define B200_DTYPE_F32 2     /* b200_rotate, b200_verify_tokens   */
 
 /* Epilogue selector of b200_qmm_fused. */
 #define B200_EPI_NONE 0      /* y = fp16(acc) [+ bias, in fp16]                               */
@@ -497,6 +499,77 @@ int b200_logits_rowstats_temp(const void* logits, int R, int V, uint32_t* row_ma
 /* accept_candidate (mlx_eagle.py:349-376) over all layers; cache is [layers][2][Hkv][cache_rows][hd]. */
 int b200_kv_compact(void* cache, int layers, int Hkv, int cache_rows, int hd, const int* accept_rows,
                     const int* ctl, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Rotary positions in general form, a paged cache with a prefix that requests share, and the verification of drafted tokens
+ * against given probabilities.  No counterpart in the reference, which has one request, one contiguous cache and greedy acceptance.
+ * Strides are in elements; the last dimension (head size, vocabulary) is contiguous everywhere.
+ * ------------------------------------------------------------------------------------------ */
+
+/* Rotation by theta = position * scaling * inv_freqs[i]: (a, b) -> magnitude * (a cos - b sin, a sin + b cos) for the pairs (x[i],
+ * x[i + rotary_dim / 2]) or, interleaved, (x[2 i], x[2 i + 1]).  Dims from rotary_dim on pass through.  The angle is the product of the
+ * numbers given, whatever the position: it is reduced to a turn in whole numbers. */
+typedef struct b200_rotary {
+    const void* positions;      /* [tokens] int32, or int64 */
+    const float* inv_freqs;     /* [rotary_dim / 2] */
+    double scaling;
+    float magnitude;
+    int positions_64;
+    int rotary_dim;             /* even, at most the head size */
+    int interleaved;
+    int inverse;                /* by -theta: the gradient of the rotation, or positions taken out again (magnitude is not) */
+} b200_rotary;
+
+/* out[t][h] = x[t][h] rotated; out may be x.  dtype F16, BF16 or F32; dim at most 2048, heads 65535. */
+int b200_rotate(const b200_rotary* r, const void* x, long long x_token, long long x_head, void* out, long long out_token, long long out_head,
+                int dtype, int tokens, int heads, int dim, void* stream);
+
+/* A pass of several requests over a cache of pages.  Row r of request b is row r % page_size of page page_table[b][r / page_size].
+ * The pass's tokens row_starts[b] .. row_starts[b + 1] - 1 are the last of the request's `lengths[b]` rows, themselves among them; tokens
+ * ahead of row_starts[0] or from row_starts[requests] on are nobody's.  row_starts ascends and ends at `tokens` or below.  Tables and lengths
+ * are read on the device: nothing here depends on their values at the time of the call. */
+typedef struct b200_paged {
+    int dtype;                  /* of q, k, v, pages and results: F16 or BF16 */
+    int requests, tokens;
+    int heads, kv_heads, head_dim;
+    int pages, page_size, table_width;
+    const int* page_table;      /* [requests][table_width] */
+    long long table_stride;
+    const int* lengths;         /* [requests] */
+    const int* row_starts;      /* [requests + 1] */
+    void* k_pages;              /* [pages][kv_heads][page_size][head_dim] in any order of strides */
+    void* v_pages;              /* with the same strides */
+    long long page_stride, head_stride, row_stride;
+} b200_paged;
+
+/* k, v -> cache rows, k rotated; q_out = q rotated (may be q), in one launch.  Positions are r->positions, or with NULL the token's row behind
+ * `prefix_length` rows.  A row whose page number is outside the cache, or that the table is too short for, is not written; tokens that are
+ * nobody's are left alone, in q_out too.  r->inverse must be 0. */
+int b200_paged_append(const b200_paged* c, const b200_rotary* r, const void* q, long long q_token, long long q_head, const void* k, const void* v,
+                      long long kv_token, long long kv_head, void* q_out, long long out_token, long long out_head, int prefix_length, void* stream);
+
+/* out[t][h] = softmax(scale * q . K) V over the rows of the shared prefix (prefix_pages, prefix_length rows; NULL and 0: none) and those of
+ * the token's own request: causal, or by `mask`: one word a token, bit j = the token sees the request's j-th new row (rows from the 64th
+ * on are hidden); older rows are seen by all.  A token that sees nothing gets zeros; tokens that are nobody's are left alone.  Rows behind the
+ * last may hold anything; a page number outside the cache stands for rows of zeros.  head_dim 64 or 128; page_size 8, 16, 32, 64 or a multiple of
+ * 128; strides multiples of 8, pointers 16-byte aligned; at most 1024 requests.
+ * workspace: b200_paged_attention_workspace_bytes(c) bytes, 16-byte aligned, of any content, not shared with a call that may run at the same
+ * time.  error: device word, zero at first; not zero after a wait inside the kernel that ran out. */
+size_t b200_paged_attention_workspace_bytes(const b200_paged* c);
+int b200_paged_attention(const b200_paged* c, const void* q, long long q_token, long long q_head, void* out, long long out_token, long long out_head,
+                         const int* prefix_pages, int prefix_length, const unsigned long long* mask, float scale, void* workspace,
+                         size_t workspace_bytes, int* error, void* stream);
+
+/* Speculative sampling from given random numbers.  Drafted token i of a request stands while uniforms[i] * q_i(x_i) < p_i(x_i) and all before
+ * it do; the token behind the n that stand is drawn by uniforms[drafts] from max(p_n - q_n, 0) (refused) or p_n (all stand): the lowest j whose sum
+ * of weights 0..j exceeds uniforms[drafts] times the sum of all, in 64 bits.  Where p_n - q_n leaves nothing it is drawn from p_n, and where that
+ * is empty it is token 0.  target: [requests][drafts + 1][vocab] probabilities (need not sum to one); draft: [requests][drafts][vocab], or NULL for
+ * drafts that were not drawn (q = 1 at the token); draft_lengths: [requests] drafts in use, or NULL for all.  A drafted token outside
+ * the vocabulary is refused.  tokens_out: [requests][drafts + 1], the tokens that stand, the drawn one, then -1; accepted: [requests].
+ * dtype (both distributions) F16, BF16 or F32; drafts at most 1024, vocab 2^30, requests 65535. */
+int b200_verify_tokens(const int* draft_tokens, long long tokens_stride, const void* target, long long target_request, long long target_row,
+                       const void* draft, long long draft_request, long long draft_row, const float* uniforms, long long uniforms_stride,
+                       const int* draft_lengths, int dtype, int requests, int drafts, int vocab, int* tokens_out, int* accepted, void* stream);
 
 #ifdef __cplusplus
 }

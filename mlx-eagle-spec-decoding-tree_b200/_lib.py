@@ -7,6 +7,7 @@ torch; the library only sees raw device pointers and the current CUDA stream.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import importlib.util
 import os
@@ -74,7 +75,7 @@ def _declare(l: ctypes.CDLL) -> None:
     l.b200_qmm.argtypes = [vp] * 6 + [i32] * 5 + [vp, sz, vp]
     l.b200_qmm_fused.restype = i32
     l.b200_qmm_fused.argtypes = [vp] * 10 + [i32] * 6 + [vp, sz, vp]
-    f32, u64 = ctypes.c_float, ctypes.c_ulonglong
+    f32, u64, i64 = ctypes.c_float, ctypes.c_ulonglong, ctypes.c_longlong
     l.b200_qmm_noalloc_max_scratch_bytes.restype = sz
     l.b200_qmm_noalloc.restype = i32
     l.b200_qmm_noalloc.argtypes = [vp] * 6 + [i32] * 5 + [vp]
@@ -170,6 +171,16 @@ def _declare(l: ctypes.CDLL) -> None:
     l.b200_residual_add_f32.argtypes = [vp, vp, i32, i32, vp]
     l.b200_argmax_key_shift.restype = i32
     l.b200_argmax_key_shift.argtypes = [vp, i32, ctypes.c_uint, vp]
+    l.b200_rotate.restype = i32
+    l.b200_rotate.argtypes = [ctypes.POINTER(Rotary), vp, i64, i64, vp, i64, i64] + [i32] * 4 + [vp]
+    l.b200_paged_append.restype = i32
+    l.b200_paged_append.argtypes = [ctypes.POINTER(Paged), ctypes.POINTER(Rotary), vp, i64, i64, vp, vp, i64, i64, vp, i64, i64, i32, vp]
+    l.b200_paged_attention_workspace_bytes.restype = sz
+    l.b200_paged_attention_workspace_bytes.argtypes = [ctypes.POINTER(Paged)]
+    l.b200_paged_attention.restype = i32
+    l.b200_paged_attention.argtypes = [ctypes.POINTER(Paged), vp, i64, i64, vp, i64, i64, vp, i32, vp, f32, vp, sz, vp, vp]
+    l.b200_verify_tokens.restype = i32
+    l.b200_verify_tokens.argtypes = [vp, i64, vp, i64, i64, vp, i64, i64, vp, i64, vp] + [i32] * 4 + [vp] * 3
     l.b200_kv_compact.restype = i32
     l.b200_kv_compact.argtypes = [vp, i32, i32, i32, i32, vp, vp, vp]
 
@@ -206,6 +217,23 @@ class PrefillDesc(ctypes.Structure):
         + [("workspace_bytes", ctypes.c_size_t)])
 
 
+class Rotary(ctypes.Structure):
+    """Mirror of ``b200_rotary``."""
+    _fields_ = [("positions", ctypes.c_void_p), ("inv_freqs", ctypes.c_void_p), ("scaling", ctypes.c_double), ("magnitude", ctypes.c_float),
+                ("positions_64", ctypes.c_int), ("rotary_dim", ctypes.c_int), ("interleaved", ctypes.c_int), ("inverse", ctypes.c_int)]
+
+
+class Paged(ctypes.Structure):
+    """Mirror of ``b200_paged``."""
+    _fields_ = ([(n, ctypes.c_int) for n in ("dtype", "requests", "tokens", "heads", "kv_heads", "head_dim", "pages", "page_size", "table_width")]
+                + [("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_longlong)]
+                + [(n, ctypes.c_void_p) for n in ("lengths", "row_starts", "k_pages", "v_pages")]
+                + [(n, ctypes.c_longlong) for n in ("page_stride", "head_stride", "row_stride")])
+
+
+DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}      # B200_DTYPE_*
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         extra = ""
@@ -220,6 +248,35 @@ def ptr(t: torch.Tensor | None):
 
 def stream_ptr(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def require_tensor(what: str, t, dtypes, shape, like: torch.Tensor = None, packed: bool = True) -> None:
+    """``t`` is a CUDA tensor of one of ``dtypes`` and of ``shape`` (None: any size), on the device of ``like``; without gaps (``packed``), or
+    with a contiguous last dimension."""
+    if not isinstance(t, torch.Tensor):
+        raise B200Error(f"{what} must be a tensor")
+    require_cuda(t)
+    if t.dtype not in dtypes:
+        raise B200Error(f"{what} must be {' or '.join(str(d).removeprefix('torch.') for d in dtypes)}, not {str(t.dtype).removeprefix('torch.')}")
+    if t.dim() != len(shape) or any(want is not None and have != want for have, want in zip(t.shape, shape)):
+        raise B200Error(f"{what} must have the shape ({', '.join('*' if n is None else str(n) for n in shape)}), not {tuple(t.shape)}")
+    if packed and not t.is_contiguous():
+        raise B200Error(f"{what} must be contiguous")
+    if not packed and t.numel() > 0 and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise B200Error(f"the last dimension of {what} must be contiguous")
+    if like is not None and t.device != like.device:
+        raise B200Error(f"{what} must be on {like.device}, not {t.device}")
+
+
+def require_writable(what: str, t: torch.Tensor) -> None:
+    """No two elements of a result share their place by a stride of 0."""
+    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+        raise B200Error(f"{what} must not be expanded: its elements share their places")
+
+
+def on_device(t: torch.Tensor):
+    """The tensor's device as the current one for a launch (a context)."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def require_cuda(*tensors: torch.Tensor) -> None:

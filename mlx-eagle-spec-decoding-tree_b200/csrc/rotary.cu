@@ -1,0 +1,259 @@
+// Rotary positions in general form, and the append of a pass's keys and values to a paged cache with the rotation on the way.
+//
+//   theta = position * scaling * inv_freq[i];  (a, b) -> magnitude * (a cos - b sin, a sin + b cos)
+//
+// for the pairs (x[i], x[i + R/2]) or, interleaved, (x[2i], x[2i + 1]) of the first R dims; the dims behind them pass through.
+//
+// The angle is reduced in whole numbers: scaling * inv_freq / 2 pi as a 64-bit fraction of a turn, times the position modulo 2^64, is the
+// fraction of a turn of the product, whatever the position (53 bits of the product of doubles: 2^-37 turns at 131072 and a frequency of
+// one, where a product in single precision is off by 2^-9 radians).  Products and sums of a pair are fp32, rounded once to the result's type.
+#include <algorithm>
+
+#include "paged.cuh"
+#include "typed.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kRotThreads = 256;
+constexpr int kRotTokens = 4;                    // of a CTA, at most
+constexpr int kRotItems = 4;                     // loads of a thread in flight
+
+// One block of heads that share addresses: head h of token t at base + t * token + h * head (elements).
+struct Heads {
+    char* base;
+    long long token, head;
+};
+
+struct RotParams {
+    Heads in, out;                               // queries of the append
+    Heads k, v;                                  // the append's new rows
+    char *k_pages, *v_pages;
+    long long page_stride, page_head, page_row;  // elements
+    const void* positions;                       // or NULL: row in the request, behind the prefix
+    int pos64;
+    const float* inv_freqs;
+    double turns;                                // scaling / 2 pi
+    float magnitude;
+    int inverse;
+    int tokens, heads, kv_heads, dim, half;      // half: pairs that are rotated
+    int per_cta;                                 // tokens of a CTA
+    // append
+    const int *table, *lengths, *row_starts;
+    long long table_stride;
+    int requests, pages, page_size, table_width, prefix;
+};
+
+// Largest r with starts[r] <= t, by the lanes of a warp (starts ascending, starts[0] <= t).
+__device__ __forceinline__ int find_request(const int* starts, int requests, int t, int lane) {
+    int lo = 0, hi = requests;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
+        const int n = __popc(__ballot_sync(0xffffffffu, at < hi && starts[at] <= t));
+        lo += n * step;
+        hi = min(hi, lo + step);
+    }
+    return lo;
+}
+
+// An item is VE dims of one head (interleaved: VE / 2 pairs), or the VE pairs of two times VE dims.  WHOLE: all loads are of 16 bytes; else element
+// by element, for any strides and sizes.  What bounds it: launch latency up to a few MB, then HBM.
+template <typename T, int VE, bool WHOLE, bool INTERLEAVED, bool APPEND>
+__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotParams p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    extern __shared__ float2 turned[];                                   // [token][half]: magnitude * (cos, sin)
+    __shared__ long long s_pos[kRotTokens], s_row[kRotTokens];           // position; cache offset, -1: nowhere, -2: no request's token
+    const int t0 = blockIdx.x * p.per_cta, toks = min(p.per_cta, p.tokens - t0);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (warp < toks) {
+        const int t = t0 + warp;
+        long long row = 0, at = 0;
+        if (APPEND) {
+            at = -2;
+            if (t >= p.row_starts[0] && t < p.row_starts[p.requests]) {
+                const int r = find_request(p.row_starts, p.requests, t, lane);
+                row = (long long)p.lengths[r] - p.row_starts[r + 1] + t;
+                at = -1;
+                if (row >= 0 && row < (long long)p.table_width * p.page_size) {
+                    const int page = p.table[r * p.table_stride + row / p.page_size];
+                    if (page >= 0 && page < p.pages) at = page * p.page_stride + row % p.page_size * p.page_row;
+                }
+            }
+        }
+        if (lane == 0) {
+            s_row[warp] = at;
+            s_pos[warp] = p.positions == nullptr ? row + p.prefix
+                                                 : (p.pos64 ? static_cast<const long long*>(p.positions)[t] : (long long)static_cast<const int*>(p.positions)[t]);
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < toks * p.half; i += kRotThreads) {
+        const int t = i / p.half;
+        double f = p.inv_freqs[i - t * p.half] * p.turns;
+        f -= floor(f);
+        const unsigned long long phase = __double2ull_rz(f * 0x1p64) * (unsigned long long)s_pos[t];
+        const unsigned quarter = (unsigned)((phase + (1ull << 61)) >> 62);                   // the nearest quarter of a turn, what is left to either side
+        float s, c;
+        sincospif((float)(long long)(phase - ((unsigned long long)quarter << 62)) * 0x1p-63f, &s, &c);
+        if (quarter & 1) {
+            const float x = s;
+            s = c;
+            c = -x;
+        }
+        if (quarter & 2) {
+            s = -s;
+            c = -c;
+        }
+        turned[i] = make_float2(c * p.magnitude, (p.inverse ? -s : s) * p.magnitude);
+    }
+    __syncthreads();
+
+    const int rot = p.half * 2, pair_items = ((INTERLEAVED ? rot : p.half) + VE - 1) / VE;
+    const int head_items = pair_items + (p.dim - rot + VE - 1) / VE;
+    const int heads = APPEND ? p.heads + 2 * p.kv_heads : p.heads, total = toks * heads * head_items;
+    const int stride = gridDim.y * kRotThreads;
+    for (int first = blockIdx.y * kRotThreads + threadIdx.x; first < total; first += stride * kRotItems) {
+        Vec<T, VE> a[kRotItems], b[kRotItems];
+        T* dst[kRotItems];
+        const float2* cs[kRotItems];                                     // NULL: passes through
+        int n[kRotItems];                                                // elements; negative: of either side
+#pragma unroll
+        for (int j = 0; j < kRotItems; j++) {
+            const int i = first + j * stride;
+            dst[j] = nullptr;
+            cs[j] = nullptr;
+            n[j] = 0;
+            if (i >= total) continue;
+            const int hd = i / head_items, it = i - hd * head_items, t = hd / heads;
+            int h = hd - t * heads;
+            const Heads* from = &p.in;
+            char* base = p.out.base;
+            long long to;
+            bool turn = it < pair_items;
+            if (!APPEND || h < p.heads) {
+                if (APPEND && s_row[t] == -2) continue;
+                to = (t0 + t) * p.out.token + h * p.out.head;
+            } else {
+                if (s_row[t] < 0) continue;
+                const bool is_k = h < p.heads + p.kv_heads;
+                h -= is_k ? p.heads : p.heads + p.kv_heads;
+                from = is_k ? &p.k : &p.v;
+                base = is_k ? p.k_pages : p.v_pages;
+                to = s_row[t] + h * p.page_head;
+                turn = turn && is_k;
+            }
+            const bool paired = !INTERLEAVED && it < pair_items;
+            const int c = it < pair_items ? it * VE : rot + (it - pair_items) * VE, left = (it >= pair_items ? p.dim : (INTERLEAVED ? rot : p.half)) - c;
+            const T* src = reinterpret_cast<const T*>(from->base) + (t0 + t) * from->token + h * from->head + c;
+            n[j] = paired ? -min(left, VE) : min(left, VE);
+            load_vec<WHOLE>(a[j], src, min(left, VE));
+            if (paired) load_vec<WHOLE>(b[j], src + p.half, min(left, VE));
+            dst[j] = reinterpret_cast<T*>(base) + to + c;
+            if (turn) cs[j] = turned + t * p.half + (INTERLEAVED ? c / 2 : c);
+        }
+#pragma unroll
+        for (int j = 0; j < kRotItems; j++) {
+            if (dst[j] == nullptr) continue;
+            const int count = abs(n[j]);
+            if (cs[j] != nullptr) {
+#pragma unroll
+                for (int e = 0; e < VE; e += INTERLEAVED ? 2 : 1) {
+                    if (!WHOLE && e >= count) break;
+                    const float2 w = cs[j][INTERLEAVED ? e / 2 : e];
+                    T& lo = a[j].v[e];
+                    T& hi = INTERLEAVED ? a[j].v[(e + 1) % VE] : b[j].v[e];
+                    const float x = to_f32(lo), y = to_f32(hi);
+                    lo = from_f32<T>(x * w.x - y * w.y);
+                    hi = from_f32<T>(x * w.y + y * w.x);
+                }
+            }
+            store_vec<WHOLE>(dst[j], a[j], count);
+            if (n[j] < 0) store_vec<WHOLE>(dst[j] + p.half, b[j], count);
+        }
+    }
+}
+
+// Whether all rows start at 16 bytes and their pieces are whole loads.
+bool whole(const RotParams& p, const Heads& h, int ve) { return aligned16(h.base) && h.token % ve == 0 && h.head % ve == 0; }
+
+template <typename T, bool APPEND>
+int launch_rotary(RotParams& p, bool interleaved, cudaStream_t stream) {
+    constexpr int VE = 16 / sizeof(T);
+    const int rot = 2 * p.half;
+    bool vec = p.dim % VE == 0 && (interleaved ? rot : p.half) % VE == 0 && whole(p, p.in, VE) && whole(p, p.out, VE);
+    if (APPEND)
+        vec = vec && whole(p, p.k, VE) && whole(p, p.v, VE) && aligned16(p.k_pages) && aligned16(p.v_pages) && p.page_stride % VE == 0 &&
+              p.page_head % VE == 0 && p.page_row % VE == 0;
+    const int ve = vec ? VE : 2, heads = APPEND ? p.heads + 2 * p.kv_heads : p.heads;
+    const int items = heads * (((interleaved ? rot : p.half) + ve - 1) / ve + (p.dim - rot + ve - 1) / ve);
+    // Tokens of a CTA: so many that every thread has its loads in flight, as long as there are CTAs for all SMs; a token of many heads
+    // goes to several, whose number of waves counts the angles' share.
+    p.per_cta = 1;
+    while (p.per_cta < kRotTokens && p.per_cta * items < kRotThreads * kRotItems && p.tokens / (2 * p.per_cta) >= 2 * 148) p.per_cta *= 2;
+    const int split = p.tokens >= 2 * 148 ? kRotItems : 1;               // (few tokens: a load a thread)
+    const int gy = std::min((p.per_cta * items + kRotThreads * split - 1) / (kRotThreads * split), 256);
+    const dim3 grid((p.tokens + p.per_cta - 1) / p.per_cta, gy);
+    const size_t smem = sizeof(float2) * p.half * p.per_cta;
+    auto go = [&](auto kern) { launch_kernel(kern, grid, dim3(kRotThreads), smem, stream, p); };
+    if (vec) {
+        if (interleaved) go(rotary_kernel<T, VE, true, true, APPEND>);
+        else go(rotary_kernel<T, VE, true, false, APPEND>);
+    } else if (interleaved) {
+        go(rotary_kernel<T, 2, false, true, APPEND>);
+    } else {
+        go(rotary_kernel<T, 2, false, false, APPEND>);
+    }
+    return check_launch();
+}
+
+constexpr double kTwoPi = 6.283185307179586476925286766559;
+
+}  // namespace
+}  // namespace b200
+
+extern "C" {
+
+int b200_rotate(const b200_rotary* r, const void* x, long long x_token, long long x_head, void* out, long long out_token, long long out_head,
+                int dtype, int tokens, int heads, int dim, void* stream) {
+    if (!r || tokens < 0 || heads < 0 || dim < 1 || dim > 2048) return B200_EINVAL;
+    if (r->rotary_dim < 2 || (r->rotary_dim & 1) || r->rotary_dim > dim) return B200_EINVAL;
+    if (b200::dtype_size(dtype) == 0) return B200_EUNSUPPORTED;
+    if (tokens == 0 || heads == 0) return B200_OK;
+    if (!x || !out || !r->positions || !r->inv_freqs || heads > 65535) return B200_EINVAL;
+    b200::RotParams p{};
+    p.in = {static_cast<char*>(const_cast<void*>(x)), x_token, x_head};
+    p.out = {static_cast<char*>(out), out_token, out_head};
+    p.positions = r->positions; p.pos64 = r->positions_64; p.inv_freqs = r->inv_freqs; p.turns = r->scaling / b200::kTwoPi;
+    p.magnitude = r->magnitude; p.inverse = r->inverse; p.tokens = tokens; p.heads = heads; p.dim = dim; p.half = r->rotary_dim / 2;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == B200_DTYPE_F32) return b200::launch_rotary<float, false>(p, r->interleaved, st);
+    if (dtype == B200_DTYPE_BF16) return b200::launch_rotary<__nv_bfloat16, false>(p, r->interleaved, st);
+    return b200::launch_rotary<__half, false>(p, r->interleaved, st);
+}
+
+int b200_paged_append(const b200_paged* c, const b200_rotary* r, const void* q, long long q_token, long long q_head, const void* k, const void* v,
+                      long long kv_token, long long kv_head, void* q_out, long long out_token, long long out_head, int prefix_length, void* stream) {
+    const int bad = b200::check_paged(c);
+    if (bad != B200_OK) return bad;
+    if (!r || r->rotary_dim < 2 || (r->rotary_dim & 1) || r->rotary_dim > c->head_dim || prefix_length < 0 || r->inverse) return B200_EINVAL;
+    if (c->tokens == 0 || c->requests == 0) return B200_OK;
+    if (!q || !k || !v || !q_out || !r->inv_freqs) return B200_EINVAL;
+    b200::RotParams p{};
+    p.in = {static_cast<char*>(const_cast<void*>(q)), q_token, q_head};
+    p.k = {static_cast<char*>(const_cast<void*>(k)), kv_token, kv_head};
+    p.v = {static_cast<char*>(const_cast<void*>(v)), kv_token, kv_head};
+    p.out = {static_cast<char*>(q_out), out_token, out_head};
+    p.k_pages = static_cast<char*>(c->k_pages); p.v_pages = static_cast<char*>(c->v_pages);
+    p.page_stride = c->page_stride; p.page_head = c->head_stride; p.page_row = c->row_stride;
+    p.positions = r->positions; p.pos64 = r->positions_64; p.inv_freqs = r->inv_freqs; p.turns = r->scaling / b200::kTwoPi;
+    p.magnitude = r->magnitude;
+    p.tokens = c->tokens; p.heads = c->heads; p.kv_heads = c->kv_heads; p.dim = c->head_dim; p.half = r->rotary_dim / 2;
+    p.table = c->page_table; p.lengths = c->lengths; p.row_starts = c->row_starts; p.table_stride = c->table_stride;
+    p.requests = c->requests; p.pages = c->pages; p.page_size = c->page_size; p.table_width = c->table_width; p.prefix = prefix_length;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (c->dtype == B200_DTYPE_BF16) return b200::launch_rotary<__nv_bfloat16, true>(p, r->interleaved, st);
+    return b200::launch_rotary<__half, true>(p, r->interleaved, st);
+}
+
+}  // extern "C"

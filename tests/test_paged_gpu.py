@@ -1,0 +1,357 @@
+"""A paged cache behind a prefix that requests share: append and attention against their definitions in 64 bits.
+
+Tolerance of the attention, e = eps / 2 of the type, A = sum of p |v| per output: a probability is rounded to the type (e p), and the sum uses the
+rounded ones (e A more, after division); the result is rounded (e |o|).  Scores are fp32 sums of 16-bit products, off by at most 2^-20 of
+S = scale * sum |q k| (128 terms, 2^-24 each, and as much again for a sum that truncates), which moves a probability by twice that
+relatively (its own and the sum's), as do the roundings of exp2 and of the running sums, 2^-18 together for up to 2^14 rows.  fp16
+probabilities below 2^-14 are off by up to 2^-25 in place of e p, relative to the largest: a row of n keys by n 2^-25 max |v| at most, over a sum of
+at least 1."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+HALF, BF = torch.float16, torch.bfloat16
+
+
+class Batch:
+    """Requests with `new` tokens each behind `old` rows, pages in random order, everything that is nobody's poisoned."""
+
+    def __init__(self, cuda, heads, kv, hd, page, prefix, old, new, dtype=HALF, seed=0, order="hnd", poison=float("nan"), spread=2.0, pad=0):
+        g = torch.Generator().manual_seed(seed)
+        self.heads, self.kv, self.hd, self.page, self.prefix, self.old, self.new = heads, kv, hd, page, prefix, old, new
+        lengths = [o + n for o, n in zip(old, new)]
+        need = [(x + page - 1) // page for x in lengths]
+        shared = (prefix + page - 1) // page
+        pages = shared + sum(need) + 2
+        perm = torch.randperm(pages, generator=g).int()
+        self.prefix_pages = perm[:shared].to(cuda)
+        table = torch.full((len(old), max(need + [1]) + 1), -7, dtype=torch.int32)
+        at = shared
+        for b, n in enumerate(need):
+            table[b, :n] = perm[at:at + n]
+            at += n
+        self.table = table.to(cuda)
+        shape = (2, pages, kv, page, hd) if order == "hnd" else (2, pages, page, kv, hd)
+        data = torch.full(shape, poison).to(dtype).to(cuda)
+        self.data = data if order == "hnd" else data.transpose(2, 3)
+        self.k_pages, self.v_pages = self.data[0], self.data[1]
+        self.lengths = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+        self.row_starts = torch.tensor([sum(new[:i]) for i in range(len(new) + 1)], dtype=torch.int32, device=cuda)
+        self.tokens = sum(new) + pad
+        # dense rows: the prefix's, then each request's
+        draw = lambda n: torch.randn(2, kv, n, hd, generator=g).to(dtype).to(cuda)
+        self.shared = draw(prefix)
+        self.rows = [draw(x) for x in lengths]
+        self._put(self.prefix_pages.tolist(), self.shared)
+        for b, r in enumerate(self.rows):
+            self._put(self.table[b].tolist(), r)
+        self.q = (spread * torch.randn(self.tokens, heads, hd, generator=g)).to(dtype).to(cuda)
+        self.mask = None
+
+    def _put(self, pages, rows):
+        for i in range(0, rows.shape[2], self.page):
+            n = min(self.page, rows.shape[2] - i)
+            self.data[:, pages[i // self.page], :, :n] = rows[:, :, i:i + n]
+
+    def tree(self, seed=1, empty=False):
+        g = torch.Generator().manual_seed(seed)
+        words = []
+        for n in self.new:
+            mine = []
+            for i in range(n):
+                parent = mine[int(torch.randint(0, i, (1,), generator=g))] if i else 0
+                mine.append(parent | 1 << i)
+            words += mine
+        words += [0] * (self.tokens - len(words))
+        if empty:
+            words[::2] = [0] * len(words[::2])
+        words = [w & (1 << 64) - 1 for w in words]                       # (bits of the first 64 new rows)
+        self.mask = torch.tensor([w - (1 << 64) if w >= 1 << 63 else w for w in words], dtype=torch.int64).to(self.q.device)
+        return self
+
+    def run(self, be, **kw):
+        args = dict(prefix_pages=self.prefix_pages if self.prefix else None, prefix_length=self.prefix, mask=self.mask)
+        args.update(kw)
+        return be.paged.attention(self.q, self.k_pages, self.v_pages, self.table, self.lengths, self.row_starts, **args)
+
+    def exact(self, scale=None):
+        """(o, tolerance) in 64 bits; tokens that are nobody's are NaN."""
+        scale = self.hd ** -0.5 if scale is None else scale
+        dtype = self.q.dtype
+        e = torch.finfo(dtype).eps / 2
+        group = self.heads // self.kv
+        out = torch.full(self.q.shape, math.nan, dtype=torch.float64, device=self.q.device)
+        tol = torch.zeros_like(out)
+        at = 0
+        for b, n in enumerate(self.new):
+            if n == 0:
+                continue
+            old, rows = self.old[b], torch.cat([self.shared, self.rows[b]], 2).double()
+            k, v = rows[0].repeat_interleave(group, 0), rows[1].repeat_interleave(group, 0)              # (heads, keys, hd)
+            q = self.q[at:at + n].double().transpose(0, 1)
+            seen = torch.ones(n, rows.shape[2], dtype=torch.bool, device=self.q.device)
+            for j in range(n):
+                col = self.prefix + old + j
+                seen[:, col] = torch.arange(n, device=seen.device) >= j if self.mask is None else \
+                    (((self.mask[at:at + n] >> j) & 1 == 1) if j < 64 else torch.zeros(n, dtype=torch.bool, device=seen.device))
+            s = (scale * q @ k.transpose(1, 2)).masked_fill(~seen, -math.inf)
+            p = torch.softmax(s, -1)
+            p = torch.where(seen.any(-1)[:, None], p, torch.zeros_like(p))
+            o, a = p @ v, p @ v.abs()
+            big = float((abs(scale) * q.abs() @ k.abs().transpose(1, 2)).max()) if rows.shape[2] else 0.0
+            small = rows.shape[2] * 2.0 ** -25 * float(v.abs().max()) if dtype == HALF and rows.shape[2] else 0.0
+            out[at:at + n] = o.transpose(0, 1)
+            tol[at:at + n] = (e * o.abs() + (2 * e + 2 * 2.0 ** -20 * big + 2.0 ** -18) * a).transpose(0, 1) + small + (2.0 ** -25 if dtype == HALF else 0.0)
+            at += n
+        return out, tol
+
+    def check(self, be, scale=None, **kw):
+        got = self.run(be, **({} if scale is None else dict(scale=scale)), **kw)
+        want, tol = self.exact(scale)
+        n = sum(self.new)
+        assert got.dtype == self.q.dtype
+        bad = ~((got[:n].double() - want[:n]).abs() <= tol[:n])
+        assert not bad.any(), (int(bad.sum()), bad.nonzero()[0].tolist(), got[:n][bad][:4].tolist(), want[:n][bad][:4].tolist())
+        assert be.paged.attention_error(self.q.device) == 0
+        return got
+
+
+SHAPES = [(14, 2, 64), (8, 2, 128), (9, 3, 128), (4, 4, 64), (32, 1, 128), (160, 1, 64)]
+BATCHES = [
+    # prefix, old rows, new tokens
+    (0, [0], [1]),
+    (0, [5, 0, 127, 128, 129], [1, 1, 1, 1, 1]),
+    (1, [0, 0], [1, 3]),
+    (127, [3], [2]),
+    (128, [1000, 0, 64], [1, 7, 0]),
+    (129, [0, 250], [130, 2]),
+    (1000, [700] * 9, [1] * 9),
+    (4099, [10, 300, 0, 45, 1], [1, 2, 33, 16, 5]),
+    (700, [0] * 40, [4] * 40),
+    (20000, [100, 2500], [1, 1]),
+]
+
+
+@pytest.mark.parametrize("batch", BATCHES, ids=lambda b: f"{b[0]}-{len(b[1])}x{max(b[2])}")
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_attention_is_the_definition(be, cuda, shape, batch):
+    dtype = BF if len(batch[1]) % 2 else HALF
+    Batch(cuda, *shape, 16, *batch, dtype=dtype).check(be)
+    Batch(cuda, *shape, 128, *batch, dtype=HALF if dtype == BF else BF, order="nhd", seed=1).check(be)
+
+
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 256, 384])
+@pytest.mark.parametrize("order", ["hnd", "nhd"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_pages_of_any_size_and_order(be, cuda, page, order, hd):
+    Batch(cuda, 8, 2, hd, page, 777, [3, 515, 0], [1, 6, 9], order=order).check(be)
+
+
+@pytest.mark.parametrize("dtype", [HALF, BF], ids=str)
+@pytest.mark.parametrize("prefix,old,new", [(0, [0, 7, 130], [5, 64, 31]), (300, [100, 0], [64, 17]), (513, [65, 126, 1], [3, 64, 2]), (0, [40], [90])])
+@pytest.mark.parametrize("shape", [(14, 2, 64), (8, 2, 128)], ids=lambda s: "x".join(map(str, s)))
+def test_masks_of_drafted_trees(be, cuda, shape, prefix, old, new, dtype):
+    Batch(cuda, *shape, 32, prefix, old, new, dtype=dtype).tree().check(be)
+    got = Batch(cuda, *shape, 32, prefix, old, new, dtype=dtype).tree(empty=True).check(be)
+    if prefix == 0 and old[0] == 0:
+        assert (got[0] == 0).all()                                       # a token that sees nothing
+
+
+@pytest.mark.parametrize("spread,scale", [(30.0, None), (2.0, 1.0), (2.0, 0.0), (2.0, -0.1)])
+def test_peaked_flat_and_negative_scales(be, cuda, spread, scale):
+    for dtype in (HALF, BF):
+        Batch(cuda, 8, 2, 128, 16, 600, [50, 600], [3, 2], dtype=dtype, spread=spread).check(be, scale=scale)
+
+
+def test_growing_scores_leave_earlier_maxima_far_behind(be, cuda):
+    b = Batch(cuda, 8, 2, 64, 16, 2000, [900, 10], [2, 40])
+    ramp = lambda n: torch.linspace(0.1, 4.0, n, device=cuda)[:, None]
+    b.shared[0] = (b.shared[0].float().abs() * ramp(2000)).half()
+    for r in b.rows:
+        r[0] = (r[0].float().abs() * 2 * ramp(r.shape[2])).half()
+    b._put(b.prefix_pages.tolist(), b.shared)
+    for i, r in enumerate(b.rows):
+        b._put(b.table[i].tolist(), r)
+    b.q = b.q.abs()
+    b.check(be)
+
+
+def test_a_prefix_counts_like_rows_of_its_own(be, cuda):
+    """The same keys as a shared prefix, and copied into every request's pages: the same within two roundings."""
+    a = Batch(cuda, 8, 2, 128, 16, 333, [20, 90], [2, 5])
+    b = Batch(cuda, 8, 2, 128, 16, 0, [353, 423], [2, 5], seed=1)
+    for i, r in enumerate(b.rows):
+        r.copy_(torch.cat([a.shared, a.rows[i]], 2))
+        b._put(b.table[i].tolist(), r)
+    b.q = a.q
+    got = a.check(be), b.check(be)
+    _, tol = a.exact()
+    assert ((got[0].double() - got[1].double()).abs() <= 2 * tol).all()
+
+
+def test_padding_is_left_alone_and_strided_operands_are_taken(be, cuda):
+    b = Batch(cuda, 8, 2, 128, 16, 100, [20, 0, 90], [2, 0, 5], pad=4)
+    wide = torch.zeros(b.tokens, 12, 256, dtype=HALF, device=cuda)
+    wide[:, 2:10, :128] = b.q
+    b.q = wide[:, 2:10, :128]
+    out = torch.full((8, b.tokens, 128), 7.0, dtype=HALF, device=cuda).transpose(0, 1)
+    assert b.check(be, out=out) is out
+    assert (out[7:] == 7.0).all()
+    b.row_starts += 2                                                     # tokens ahead of the first request are nobody's either
+    b.q = torch.cat([b.q[:2], b.q[:9]])
+    out = torch.full((11, 8, 128), 7.0, dtype=HALF, device=cuda)
+    b.run(be, out=out)
+    assert (out[:2] == 7.0).all() and (out[9:] == 7.0).all() and (out[2:9] != 7.0).all()
+
+
+def test_page_numbers_outside_the_cache_stand_for_zeros(be, cuda):
+    b = Batch(cuda, 8, 2, 64, 16, 64, [100], [1])
+    want = Batch(cuda, 8, 2, 64, 16, 64, [100], [1])
+    want.rows[0][:, :, 16:32] = 0
+    want.rows[0][:, :, 64:80] = 0
+    want.shared[:, :, 32:48] = 0
+    b.shared, b.rows = want.shared, want.rows
+    b.table[0, 1], b.table[0, 4], b.prefix_pages[2] = b.k_pages.shape[0], -1, 2 ** 31 - 1
+    b.check(be)
+    b.lengths.fill_(-5)                                                   # no rows, as the lengths say: the prefix is left
+    b.run(be)
+    b.lengths.fill_(10 ** 6)                                              # more rows than the table has: those it has
+    assert b.run(be).isfinite().all()
+
+
+def test_append_then_attention_is_a_step(be, cuda):
+    """Steps of several requests, captured once and replayed with other lengths, against attention over the rows in 64 bits; rows the pass
+    does not write stay as they are."""
+    heads, kv, hd, page, prefix, B, T = 8, 2, 128, 16, 200, 3, 4
+    g = torch.Generator(device=cuda).manual_seed(0)
+    cache = be.PagedKVCache(2, 64, page, kv, hd, device=cuda)
+    shared = cache.take(prefix)
+    own = [cache.take(100) for _ in range(B)]
+    prefix_pages, table = torch.tensor(shared, dtype=torch.int32, device=cuda), torch.tensor(own, dtype=torch.int32, device=cuda)
+    cache.data.normal_(generator=g)
+    inv, scaling, mag = be.rope.frequencies(hd, 1e4, dict(type="yarn", factor=4.0, original_max_position_embeddings=4096), device=cuda)
+    lengths = torch.tensor([4, 20, 61], dtype=torch.int32, device=cuda)
+    starts = torch.arange(0, B * T + 1, T, dtype=torch.int32, device=cuda)
+    qkv = torch.randn(B * T, heads + 2 * kv, hd, device=cuda, generator=g).half()
+    kw = dict(scaling_factor=scaling, magnitude=mag)
+
+    def step():
+        out = []
+        for layer in range(2):
+            k_pages, v_pages = cache.layer(layer)
+            q = be.paged.append(qkv[:, :heads], qkv[:, heads:heads + kv], qkv[:, heads + kv:], k_pages, v_pages, table, lengths, starts, inv, prefix_length=prefix, **kw)
+            out.append((q, be.paged.attention(q, k_pages, v_pages, table, lengths, starts, prefix_pages=prefix_pages, prefix_length=prefix)))
+        return out
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for turn in range(3):
+        qkv.normal_(generator=g)
+        before, old = cache.data.clone(), lengths.tolist()
+        graph.replay()
+        pos = torch.cat([torch.arange(prefix + n - T, prefix + n) for n in old]).to(cuda)
+        for layer, (q, o) in enumerate(out):
+            assert torch.equal(q, be.rope.rotate(qkv[:, :heads], pos, inv, **kw))
+            kr, want = be.rope.rotate(qkv[:, heads:heads + kv], pos, inv, **kw), before[layer].clone()
+            for b in range(B):
+                for j in range(T):
+                    r = old[b] - T + j
+                    want[0, own[b][r // page], :, r % page] = kr[b * T + j]
+                    want[1, own[b][r // page], :, r % page] = qkv[b * T + j, heads + kv:]
+            assert torch.equal(cache.data[layer], want)
+            m = Batch(cuda, heads, kv, hd, page, prefix, [n - T for n in old], [T] * B)
+            rows = lambda pages, n: want[:, pages].transpose(2, 3).reshape(2, -1, kv, hd)[:, :n].transpose(1, 2)
+            m.shared, m.rows, m.q = rows(shared, prefix), [rows(own[b], old[b]) for b in range(B)], q
+            exact, tol = m.exact()
+            assert ((o.double() - exact).abs() <= tol).all()
+        lengths += T
+    cache.give(shared)
+    with pytest.raises(be._lib.B200Error):
+        cache.give(shared)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [HALF, BF], ids=str)
+@pytest.mark.parametrize("hd,rotary,page,order", [(64, 64, 16, "hnd"), (128, 64, 8, "nhd"), (96, 40, 32, "hnd"), (70, 6, 128, "nhd"), (128, 128, 64, "hnd")])
+def test_append_writes_its_rows_and_no_other(be, cuda, hd, rotary, page, order, dtype, interleaved):
+    g = torch.Generator().manual_seed(hd)
+    new = [1, 0, 40, 3, 700]
+    old = [0, 9, 100, 15, 4]
+    heads, kv, B, pad = 6, 2, 5, 3
+    b = Batch(cuda, heads, kv, hd, page, 0, old, new, dtype=dtype, order=order, poison=3.0, pad=pad)
+    b.data.copy_(torch.randn(b.data.shape, generator=g))
+    qkv = torch.randn(b.tokens, heads + 2 * kv, hd, generator=g).to(dtype).to(cuda)
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv], qkv[:, heads + kv:]
+    inv, _, _ = be.rope.frequencies(rotary, 5e5, device=cuda)
+    n = sum(new)
+    rows = torch.cat([torch.arange(o, o + x) for o, x in zip(old, new)]).to(cuda)
+    for positions, prefix in ((None, 1000), (torch.randint(0, 9999, (b.tokens,), generator=g).to(cuda), 0), (torch.arange(b.tokens, device=cuda).int(), 5)):
+        before = b.data.clone()
+        out = torch.full(q.shape, 7.0, dtype=dtype, device=cuda)
+        be.paged.append(q, k, v, b.k_pages, b.v_pages, b.table, b.lengths, b.row_starts, inv, positions=positions, prefix_length=prefix, magnitude=0.75,
+                        interleaved=interleaved, q_out=out)
+        pos = rows + prefix if positions is None else positions[:n].long()
+        kw = dict(magnitude=0.75, interleaved=interleaved)
+        assert torch.equal(out[:n], be.rope.rotate(q[:n], pos, inv, **kw)) and (out[n:] == 7.0).all()
+        kr = be.rope.rotate(k[:n], pos, inv, **kw)
+        req = torch.repeat_interleave(torch.arange(B), torch.tensor(new)).to(cuda)
+        at = b.table[req, rows // page].long()
+        before[0][at, :, rows % page] = kr
+        before[1][at, :, rows % page] = v[:n]
+        assert torch.equal(b.data, before)
+    same = qkv.clone()
+    got = be.paged.append(same[:, :heads], k, v, b.k_pages, b.v_pages, b.table, b.lengths, b.row_starts, inv, q_out=same[:, :heads], interleaved=interleaved)
+    assert torch.equal(got[:n], be.rope.rotate(q[:n], rows, inv, interleaved=interleaved)) and torch.equal(same[:, heads:], qkv[:, heads:])
+
+
+def test_append_drops_rows_without_a_page(be, cuda):
+    b = Batch(cuda, 4, 2, 64, 16, 0, [14, 0, 30], [4, 2, 6])
+    inv, _, _ = be.rope.frequencies(64, device=cuda)
+    k = torch.randn(12, 2, 64, device=cuda).half()
+    b.data.zero_()
+    b.table[0, 1] = b.k_pages.shape[0]                                    # request 0: two of four rows dropped
+    b.table[1, 0] = -1                                                    # request 1: both
+    b.lengths[2] = 10 ** 9                                                # request 2: behind the table's end
+    out = be.paged.append(b.q, k, k, b.k_pages, b.v_pages, b.table, b.lengths, b.row_starts, inv)
+    assert out.isfinite().all()
+    assert int((b.data[1] != 0).any(-1).any(1).sum()) == 2
+    b.lengths.fill_(1)                                                    # fewer rows than new tokens: what lies ahead of row 0 is dropped
+    b.data.zero_()
+    b.table.fill_(0)
+    be.paged.append(b.q, k, k, b.k_pages, b.v_pages, b.table[:, :1], b.lengths, b.row_starts, inv)
+    assert int((b.data[1] != 0).any(-1).any(1).sum()) == 1
+
+
+def test_paged_refusals(be, cuda):
+    b = Batch(cuda, 4, 2, 64, 16, 20, [14, 0], [4, 2])
+    E, at, ap = be._lib.B200Error, be.paged.attention, be.paged.append
+    inv, _, _ = be.rope.frequencies(64, device=cuda)
+    k = torch.randn(6, 2, 64, device=cuda).half()
+    base = [b.q, b.k_pages, b.v_pages, b.table, b.lengths, b.row_starts]
+
+    def changed(i, t):
+        return base[:i] + [t] + base[i + 1:]
+
+    calls = [lambda: at(*changed(0, b.q.cpu())), lambda: at(*changed(0, b.q.bfloat16())), lambda: at(*changed(0, b.q[0])), lambda: at(*changed(0, b.q[:, :3])),
+             lambda: at(*changed(1, b.k_pages[:, :1])), lambda: at(*changed(2, b.v_pages.transpose(1, 2).contiguous().transpose(1, 2))),
+             lambda: at(*changed(3, b.table.long())), lambda: at(*changed(3, b.table[:1])), lambda: at(*changed(4, b.lengths.long())),
+             lambda: at(*changed(5, b.row_starts[:2])), lambda: at(*base, prefix_length=5), lambda: at(*base, prefix_pages=b.prefix_pages, prefix_length=33),
+             lambda: at(*base, prefix_length=-1), lambda: at(*base, mask=torch.zeros(5, dtype=torch.int64, device=cuda)),
+             lambda: at(*base, mask=torch.zeros(6, dtype=torch.int32, device=cuda)), lambda: at(*base, out=b.q[:5]), lambda: at(*base, out=b.q.float()),
+             lambda: at(*changed(0, torch.zeros(6, 4, 68, device=cuda).half()[..., 1:65])),
+             lambda: at(b.q[..., :32], b.k_pages[..., :32], b.v_pages[..., :32], *base[3:]),
+             lambda: at(b.q, b.k_pages[:, :, :12], b.v_pages[:, :, :12], *base[3:]),
+             lambda: ap(b.q, k[:5], k, *base[1:], inv), lambda: ap(b.q, k, k[:, :1], *base[1:], inv), lambda: ap(b.q, k, k, *base[1:], inv[:0]),
+             lambda: ap(b.q, k, k, *base[1:], inv, prefix_length=-1), lambda: ap(b.q, k, k, *base[1:], inv, positions=torch.zeros(5, device=cuda).int()),
+             lambda: ap(b.q, k, k, *base[1:], inv, q_out=b.q[:5]), lambda: be.PagedKVCache(1, 4, 24, 2, 64, device=cuda)]
+    for call in calls:
+        with pytest.raises(E):
+            call()
+    empty = torch.zeros(0, 4, 64, device=cuda).half()
+    none = dict(page_table=b.table[:0], lengths=b.lengths[:0], row_starts=b.row_starts[:1])
+    assert at(empty, b.k_pages, b.v_pages, **none).shape == (0, 4, 64)
