@@ -27,7 +27,7 @@ inline int make_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const 
         fn = reinterpret_cast<EncodeTiledFn>(q);
         encode.store(fn, std::memory_order_release);
     }
-    const cuuint32_t estr[3] = {1, 1, 1};
+    const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
     const CUresult r = fn(map, type, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {

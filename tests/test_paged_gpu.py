@@ -218,8 +218,8 @@ def test_page_numbers_outside_the_cache_stand_for_zeros(be, cuda):
     b.check(be)
     b.lengths.fill_(-5)                                                   # no rows, as the lengths say: the prefix is left
     b.run(be)
-    b.lengths.fill_(10 ** 6)                                              # more rows than the table has: those it has
-    assert b.run(be).isfinite().all()
+    b.lengths.fill_(10 ** 6)                                              # more rows than the table has: those it has, the poisoned ones among them
+    assert b.run(be).isnan().all() and be.paged.attention_error(cuda) == 0
 
 
 def test_append_then_attention_is_a_step(be, cuda):
