@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <climits>
+#include <cmath>
 
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
@@ -114,6 +115,179 @@ PyObject* rope_positions(PyObject* const* a, Py_ssize_t n) {
     return THPVariable_Wrap(std::move(y));
 }
 
+// A CUDA tensor of `dims` dimensions on device `dev` whose last dimension is contiguous, or NULL.
+const at::Tensor* strided(PyObject* o, int64_t dims, int dev) {
+    if (!THPVariable_Check(o)) return nullptr;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    return t.is_cuda() && t.get_device() == dev && t.dim() == dims && (t.size(-1) <= 1 || t.stride(-1) == 1) ? &t : nullptr;
+}
+
+// B200_DTYPE_* of a tensor, or -1.
+int dtype_of(const at::Tensor& t) {
+    switch (t.scalar_type()) {
+        case at::kHalf: return B200_DTYPE_F16;
+        case at::kBFloat16: return B200_DTYPE_BF16;
+        case at::kFloat: return B200_DTYPE_F32;
+        default: return -1;
+    }
+}
+
+// A CUDA tensor of this type and number of values on device `dev`, without gaps and of one dimension, or NULL.
+const at::Tensor* list_of(PyObject* o, at::ScalarType type, int64_t n, int dev) {
+    const at::Tensor* t = plain(o, type);
+    return t != nullptr && t->dim() == 1 && t->get_device() == dev && (n < 0 || t->numel() == n) ? t : nullptr;
+}
+
+int current_device() { return c10::cuda::current_device(); }
+
+bool double_arg(PyObject* o, double* v) {
+    *v = PyFloat_AsDouble(o);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        return false;
+    }
+    return true;
+}
+
+// The rotation from Python's arguments: positions (or None), inv_freqs, scaling_factor, magnitude, interleaved, inverse.
+bool rotary_args(PyObject* const* a, int64_t tokens, int64_t dim, int dev, b200_rotary* r) {
+    double magnitude;
+    if (a[0] != Py_None) {
+        const at::Tensor* pos = list_of(a[0], at::kInt, tokens, dev);
+        r->positions_64 = pos == nullptr;
+        if (pos == nullptr) pos = list_of(a[0], at::kLong, tokens, dev);
+        if (pos == nullptr) return false;
+        r->positions = pos->data_ptr();
+    }
+    const at::Tensor* inv = list_of(a[1], at::kFloat, -1, dev);
+    const int interleaved = PyObject_IsTrue(a[4]), inverse = PyObject_IsTrue(a[5]);
+    if (inv == nullptr || inv->numel() < 1 || 2 * inv->numel() > dim || !double_arg(a[2], &r->scaling) || !double_arg(a[3], &magnitude) ||
+        interleaved < 0 || inverse < 0) {
+        PyErr_Clear();
+        return false;
+    }
+    r->inv_freqs = static_cast<const float*>(inv->data_ptr());
+    r->magnitude = (float)magnitude;
+    r->rotary_dim = 2 * (int)inv->numel();
+    r->interleaved = interleaved;
+    r->inverse = inverse;
+    return true;
+}
+
+// rotate(x, positions, inv_freqs, scaling_factor, magnitude, interleaved, inverse) -> out
+PyObject* rotate(PyObject* const* a, Py_ssize_t n) {
+    if (n != 7 || a[1] == Py_None) Py_RETURN_NONE;
+    const int dev = current_device();
+    const at::Tensor* x = strided(a[0], 3, dev);
+    if (!x || dtype_of(*x) < 0 || x->numel() == 0 || x->size(0) > INT_MAX || x->size(1) > 65535 || x->size(2) > 2048) Py_RETURN_NONE;
+    b200_rotary r{};
+    if (!rotary_args(a + 1, x->size(0), x->size(2), dev, &r)) Py_RETURN_NONE;
+    at::Tensor y = at::detail::empty_cuda(x->sizes(), x->scalar_type(), x->device(), c10::nullopt);
+    const int rc = b200_rotate(&r, x->data_ptr(), x->stride(0), x->stride(1), y.data_ptr(), y.stride(0), y.stride(1), dtype_of(*x), (int)x->size(0),
+                               (int)x->size(1), (int)x->size(2), stream_of(dev));
+    if (rc != B200_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(y));
+}
+
+// The pass from Python's arguments q, k_pages, v_pages, page_table, lengths, row_starts.
+const at::Tensor* paged_args(PyObject* oq, PyObject* const* a, int dev, b200_paged* c) {
+    const at::Tensor *q = strided(oq, 3, dev), *k = strided(a[0], 4, dev), *v = strided(a[1], 4, dev), *table = strided(a[2], 2, dev);
+    const at::Tensor *lengths = list_of(a[3], at::kInt, -1, dev), *starts = list_of(a[4], at::kInt, -1, dev);
+    if (!q || !k || !v || !table || !lengths || !starts || q->numel() == 0 || k->numel() == 0) return nullptr;
+    c->dtype = dtype_of(*q);
+    if ((c->dtype != B200_DTYPE_F16 && c->dtype != B200_DTYPE_BF16) || k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type() ||
+        table->scalar_type() != at::kInt || k->sizes() != v->sizes() || k->strides() != v->strides() || k->size(3) != q->size(2) ||
+        starts->numel() != lengths->numel() + 1 || table->size(0) != lengths->numel() || lengths->numel() == 0)
+        return nullptr;
+    for (int i = 0; i < 3; i++)
+        if (k->size(i) > INT_MAX || (k->size(i) > 1 && k->stride(i) == 0)) return nullptr;
+    if (q->size(0) > INT_MAX || q->size(1) > 4096 || q->size(1) % k->size(1) || q->size(2) > 2048 || table->size(1) > INT_MAX) return nullptr;
+    const int64_t page = k->size(2);
+    if (!(page == 8 || page == 16 || page == 32 || page == 64 || (page >= 128 && page % 128 == 0))) return nullptr;
+    c->requests = (int)lengths->numel(); c->tokens = (int)q->size(0); c->heads = (int)q->size(1); c->kv_heads = (int)k->size(1);
+    c->head_dim = (int)q->size(2); c->pages = (int)k->size(0); c->page_size = (int)page; c->table_width = (int)table->size(1);
+    c->page_table = static_cast<const int*>(table->data_ptr()); c->table_stride = table->stride(0);
+    c->lengths = static_cast<const int*>(lengths->data_ptr()); c->row_starts = static_cast<const int*>(starts->data_ptr());
+    c->k_pages = k->data_ptr(); c->v_pages = v->data_ptr();
+    c->page_stride = k->stride(0); c->head_stride = k->stride(1); c->row_stride = k->stride(2);
+    return q;
+}
+
+// paged_append(q, k, v, k_pages, v_pages, page_table, lengths, row_starts, prefix_length, positions, inv_freqs, scaling_factor, magnitude, interleaved,
+//              inverse) -> q_out
+PyObject* paged_append(PyObject* const* a, Py_ssize_t n) {
+    long prefix;
+    if (n != 15 || !int_arg(a[8], &prefix) || prefix < 0 || prefix > INT_MAX) Py_RETURN_NONE;
+    const int dev = current_device();
+    b200_paged c{};
+    const at::Tensor *q = paged_args(a[0], a + 3, dev, &c), *k = strided(a[1], 3, dev), *v = strided(a[2], 3, dev);
+    if (!q || !k || !v || k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type() || k->sizes() != v->sizes() ||
+        k->strides() != v->strides() || k->size(0) != c.tokens || k->size(1) != c.kv_heads || k->size(2) != c.head_dim)
+        Py_RETURN_NONE;
+    b200_rotary r{};
+    if (!rotary_args(a + 9, c.tokens, c.head_dim, dev, &r)) Py_RETURN_NONE;
+    at::Tensor y = at::detail::empty_cuda(q->sizes(), q->scalar_type(), q->device(), c10::nullopt);
+    const int rc = b200_paged_append(&c, &r, q->data_ptr(), q->stride(0), q->stride(1), k->data_ptr(), v->data_ptr(), k->stride(0), k->stride(1),
+                                     y.data_ptr(), y.stride(0), y.stride(1), (int)prefix, stream_of(dev));
+    if (rc != B200_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(y));
+}
+
+// paged_attention(q, k_pages, v_pages, page_table, lengths, row_starts, prefix_pages, prefix_length, mask, scale, error) -> out
+PyObject* paged_attention(PyObject* const* a, Py_ssize_t n) {
+    long prefix;
+    if (n != 11 || !int_arg(a[7], &prefix) || prefix < 0 || prefix > INT_MAX) Py_RETURN_NONE;
+    const int dev = current_device();
+    b200_paged c{};
+    const at::Tensor *q = paged_args(a[0], a + 1, dev, &c), *error = list_of(a[10], at::kInt, 1, dev);
+    if (!q || !error) Py_RETURN_NONE;
+    const at::Tensor* pages = a[6] == Py_None ? nullptr : list_of(a[6], at::kInt, -1, dev);
+    const at::Tensor* mask = a[8] == Py_None ? nullptr : list_of(a[8], at::kLong, c.tokens, dev);
+    double scale = std::pow((double)c.head_dim, -0.5);
+    if ((a[6] != Py_None && !pages) || (a[8] != Py_None && !mask) || (prefix > 0 && (!pages || pages->numel() * c.page_size < prefix)) ||
+        (a[9] != Py_None && !double_arg(a[9], &scale)))
+        Py_RETURN_NONE;
+    const size_t room = b200_paged_attention_workspace_bytes(&c);
+    at::Tensor y = at::detail::empty_cuda(q->sizes(), q->scalar_type(), q->device(), c10::nullopt);
+    at::Tensor ws = at::detail::empty_cuda({(int64_t)room}, at::kByte, q->device(), c10::nullopt);
+    const int rc = b200_paged_attention(&c, q->data_ptr(), q->stride(0), q->stride(1), y.data_ptr(), y.stride(0), y.stride(1),
+                                        pages ? static_cast<const int*>(pages->data_ptr()) : nullptr, (int)prefix,
+                                        mask ? static_cast<const unsigned long long*>(mask->data_ptr()) : nullptr, (float)scale, ws.data_ptr(), room,
+                                        static_cast<int*>(error->data_ptr()), stream_of(dev));
+    if (rc != B200_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(y));
+}
+
+// verify_tokens(draft_tokens, target_probs, uniforms, draft_probs, draft_lengths) -> (tokens, accepted)
+PyObject* verify_tokens(PyObject* const* a, Py_ssize_t n) {
+    if (n != 5) Py_RETURN_NONE;
+    const int dev = current_device();
+    const at::Tensor *tokens = strided(a[0], 2, dev), *p = strided(a[1], 3, dev), *u = strided(a[2], 2, dev);
+    if (!tokens || !p || !u || dtype_of(*p) < 0 || tokens->scalar_type() != at::kInt || u->scalar_type() != at::kFloat) Py_RETURN_NONE;
+    const int64_t B = p->size(0), K = p->size(1) - 1, V = p->size(2);
+    if (B < 1 || B > 65535 || K < 0 || K > 1024 || V < 1 || V > (1 << 30) || tokens->size(0) != B || tokens->size(1) != K || u->size(0) != B ||
+        u->size(1) != K + 1)
+        Py_RETURN_NONE;
+    const at::Tensor* q = a[3] == Py_None ? nullptr : strided(a[3], 3, dev);
+    const at::Tensor* lengths = a[4] == Py_None ? nullptr : list_of(a[4], at::kInt, B, dev);
+    if ((a[3] != Py_None && (!q || q->scalar_type() != p->scalar_type() || q->size(0) != B || q->size(1) != K || q->size(2) != V)) ||
+        (a[4] != Py_None && !lengths))
+        Py_RETURN_NONE;
+    at::Tensor out = at::detail::empty_cuda({B, K + 1}, at::kInt, p->device(), c10::nullopt);
+    at::Tensor accepted = at::detail::empty_cuda({B}, at::kInt, p->device(), c10::nullopt);
+    const int rc = b200_verify_tokens(static_cast<const int*>(tokens->data_ptr()), tokens->stride(0), p->data_ptr(), p->stride(0), p->stride(1),
+                                      q ? q->data_ptr() : nullptr, q ? q->stride(0) : 0, q ? q->stride(1) : 0, static_cast<const float*>(u->data_ptr()),
+                                      u->stride(0), lengths ? static_cast<const int*>(lengths->data_ptr()) : nullptr, dtype_of(*p), (int)B, (int)K, (int)V,
+                                      static_cast<int*>(out.data_ptr()), static_cast<int*>(accepted.data_ptr()), stream_of(dev));
+    if (rc != B200_OK) Py_RETURN_NONE;
+    PyObject* first = THPVariable_Wrap(std::move(out));
+    PyObject* second = THPVariable_Wrap(std::move(accepted));
+    PyObject* both = first != nullptr && second != nullptr ? PyTuple_Pack(2, first, second) : nullptr;
+    Py_XDECREF(first);
+    Py_XDECREF(second);
+    return both;
+}
+
 // layer_pointers(layers, table[, fast]) -> 0: `table` (address of [layers][8] pointers in the order of b200_forward_desc.layer_table) holds
 // the device pointers of the layers already, 1: it does now, -1: a layer is not as it should be (no re-laid-out weights, say).
 // Runs ahead of every pass, so that a pass never sees the address of a tensor that has been replaced: ~0.35 us a layer.  `fast` (address of 32
@@ -184,6 +358,8 @@ PyObject* caught(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define FAST(name, f) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST("qmm", caught<qmm>), FAST("qmm_tiled", caught<qmm_tiled>), FAST("rope_positions", caught<rope_positions>),
+                         FAST("rotate", caught<rotate>), FAST("paged_append", caught<paged_append>), FAST("paged_attention", caught<paged_attention>),
+                         FAST("verify_tokens", caught<verify_tokens>),
                          FAST("layer_pointers", layer_pointers), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_b200ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -99,6 +99,11 @@ def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Ten
     rows, or ``positions (tokens,)`` says it (a tree of drafted tokens: rows side by side, positions by depth); the rotation is
     ``rope.rotate``'s.  ``q_out`` may be ``q``.  Rows whose page number lies outside the cache, or that the table is too short for, are dropped.
     Two requests that write one page's row in the same pass leave either's."""
+    if q_out is None:
+        y = _lib.ops().paged_append(q, k, v, k_pages, v_pages, page_table, lengths, row_starts, prefix_length, positions, inv_freqs, scaling_factor,
+                                    magnitude, interleaved, False)
+        if y is not None:
+            return y
     c = _paged(q, k_pages, v_pages, page_table, lengths, row_starts)
     _lib.require_tensor("k", k, (q.dtype,), (c.tokens, c.kv_heads, c.head_dim), q, packed=False)
     _lib.require_tensor("v", v, (q.dtype,), k.shape, q, packed=False)
@@ -138,6 +143,11 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     ``q (tokens, heads, dim)``, positions already in it; heads of 64 or 128; float16 or bfloat16, scores, statistics and sums in fp32, probabilities
     rounded to the type for the second product.  ``scale`` is ``dim ** -0.5`` unless given.  A token that sees no row gets zeros.  Rows behind a
     length may hold anything; a page number outside the cache stands for rows of zeros.  At most 1024 requests."""
+    if out is None and isinstance(q, torch.Tensor):
+        y = _lib.ops().paged_attention(q, k_pages, v_pages, page_table, lengths, row_starts, prefix_pages, prefix_length, mask, scale,
+                                       _errors.get(q.device.index))
+        if y is not None:
+            return y
     c = _paged(q, k_pages, v_pages, page_table, lengths, row_starts)
     if c.head_dim not in (64, 128):
         raise _lib.B200Error(f"attention takes heads of 64 or 128 dims, not {c.head_dim}")

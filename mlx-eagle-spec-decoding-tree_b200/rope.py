@@ -101,6 +101,10 @@ def rotate(x: torch.Tensor, positions: torch.Tensor, inv_freqs: torch.Tensor, *,
 
     ``inverse`` rotates by the negative angle: the gradient of a rotation with respect to ``x`` is the rotation of the result's gradient
     with ``inverse`` and the same magnitude.  ``out`` may be ``x`` itself; other overlaps are undefined.  No gradient is recorded."""
+    if out is None:
+        y = _lib.ops().rotate(x, positions, inv_freqs, scaling_factor, magnitude, interleaved, inverse)
+        if y is not None:
+            return y
     _lib.require_tensor("x", x, tuple(_lib.DTYPES), (None, None, None), packed=False)
     tokens, heads, dim = x.shape
     if dim > 2048 or heads > 65535:

@@ -26,6 +26,9 @@ def verify_tokens(draft_tokens: torch.Tensor, target_probs: torch.Tensor, unifor
     Distributions are float32, float16 or bfloat16, both of one type, any strides but a contiguous last dimension; they need not sum to one.
     Products, differences and sums are in 64 bits.  A drafted token outside the vocabulary is refused; where ``p_n - q_n`` leaves nothing, the
     token is drawn from ``p_n``, and where that is empty it is 0.  ``K`` at most 1024."""
+    both = _lib.ops().verify_tokens(draft_tokens, target_probs, uniforms, draft_probs, draft_lengths)
+    if both is not None:
+        return both
     _lib.require_tensor("target_probs", target_probs, tuple(_lib.DTYPES), (None, None, None), packed=False)
     B, rows, V = target_probs.shape
     K = rows - 1
