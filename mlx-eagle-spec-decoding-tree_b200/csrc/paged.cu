@@ -8,10 +8,11 @@
 // an equal stretch of it, whatever the lengths: at most one piece a worker begins inside a segment, so a segment's first piece has its place by
 // (token, head) and the others theirs by worker.  A second kernel joins them.
 //
-// One CTA an SM, two workers (streams) a CTA: four warps each, a query row a thread, its scores and output in tensor memory (128 + 128 columns).  The
-// streams' blocks alternate, so that one's products run while the other's softmax does.  Where the prefix has two tiles of queries or more, the
-// CTA takes them in pairs, a tile a stream, over the same blocks: keys and values are then copied once for 256 rows.  Keys and values come page
-// by page (TMA, boxes of a page or 128 rows) into one ring in the order in which they are used.
+// One CTA an SM, two workers (streams) a CTA: eight warps each, two threads a query row, its scores and output in tensor memory (128 +
+// 128 columns); one warp issues the products of both in turn, so that one's run while the other's softmax does.  (A warp for each let both
+// streams wait for the tensor cores and for the exponentials at the same time: 4800 cycles a block of 256 rows in place of 4300.)  Where the prefix has two
+// tiles of queries or more, the CTA takes them in pairs, a tile a stream, over the same blocks: keys and values are then copied once for 256
+// rows.  Keys and values come page by page (TMA, boxes of a page or 128 rows) into one ring, blocks of the streams in turn.
 //
 // Probabilities are at most one and rounded to the type of V for the second product; scores, statistics, sums and outputs are fp32.
 // Every wait is bounded; one that runs out sets the error word and goes on.  No copy uses cluster multicast.
@@ -29,19 +30,21 @@ namespace {
 
 constexpr int kKeys = 128;                       // of a block
 constexpr int kRows = 128;                       // query rows of a tile
-constexpr int kPgThreads = 384;                  // 2 x 4 softmax warps, keys and values, products, queries of either stream
+constexpr int kParts = 2;                        // threads of a query row
+constexpr int kPgThreads = 640;                  // 2 x 8 softmax warps, keys and queries, products, values (a warp idles)
 constexpr int kPgMaxRequests = 1024;
-constexpr int kLoader = 8, kIssuer = 9, kQueries = 10;
+constexpr int kKeyLoader = 16, kIssuer = 17, kValueLoader = 18;
+constexpr float kLag = 8.f;                      // a row's maximum may exceed its reference by 2^8
 
 template <int HD>
 struct PGeo {
-    static constexpr int QTILE = kRows * HD * 2, SLOT = kKeys * HD * 2, SLOTS = HD == 128 ? 4 : 8;
-    static constexpr int KV0 = 2 * QTILE, END = KV0 + SLOTS * SLOT;
+    static constexpr int QTILE = kRows * HD * 2, SLOT = kKeys * HD * 2, SLOTS = HD == 128 ? 2 : 4;      // of keys, and of values
+    static constexpr int KV0 = 2 * QTILE, END = KV0 + 2 * SLOTS * SLOT;
     static constexpr int SMEM = END + 1024;
 };
 
 struct PagedParams {
-    CUtensorMap qmap, q1map, kmap, vmap;         // queries by tile and by token, pages
+    CUtensorMap qmap, qhmap, q1map, kmap, vmap;  // queries by tile, half a tile and token; pages
     const int *table, *lengths, *row_starts, *prefix_pages;
     const unsigned long long* mask;
     void* out;
@@ -49,7 +52,7 @@ struct PagedParams {
     float2* ml;                                  // (m, l) in the order of the pieces
     int* plan;                                   // sums of the own blocks, by request
     long long table_stride, out_token, out_head;
-    int requests, tokens, heads, kv_heads, group, tile_heads, tile_tokens, head_sets;
+    int requests, tokens, heads, kv_heads, group, tile_heads, tile_tokens, half_tokens, head_sets;
     int page_size, box_rows, table_width, prefix;
     float scale_log2;                            // positive
     bool negative;                               // ... of a negative scale
@@ -62,25 +65,34 @@ struct Line {
     int nbp;                                     // blocks of the prefix
     int tiles, pairs;                            // query tiles of the prefix, per kv head
     int odd;                                     // blocks of prefix segments without a partner
-    long long pair_total, total;                 // blocks for pairs; for single streams: odd ones, then own ones
+    int pair_total, total;                       // blocks for pairs; for single streams: odd ones, then own ones
 };
-__device__ __forceinline__ Line line_of(const PagedParams& p, long long own) {
+__device__ __forceinline__ Line line_of(const PagedParams& p, int own) {
     Line l;
     l.nbp = (p.prefix + kKeys - 1) / kKeys;
     l.tiles = (p.tokens + p.tile_tokens - 1) / p.tile_tokens * p.head_sets;
     l.pairs = l.tiles / 2;
     l.odd = l.tiles & 1 ? p.kv_heads * l.nbp : 0;
-    l.pair_total = (long long)p.kv_heads * l.pairs * l.nbp;
+    l.pair_total = p.kv_heads * l.pairs * l.nbp;
     l.total = l.odd + own;
     return l;
 }
-// Stretch of worker i of n.
-__device__ __forceinline__ long long stretch(long long total, int i, int n) { return total * i / n; }
-// The worker of n whose stretch holds block w.
-__device__ __forceinline__ int worker_of(long long total, long long w, int n) { return (int)(((w + 1) * n - 1) / total); }
+// Where the stretch of worker i of n begins (n below 2^15).
+__device__ __forceinline__ int stretch(int total, int i, int n) {
+    const int q = total / n;
+    return q * i + (total - q * n) * i / n;
+}
+// The last worker of n whose stretch begins at block w or before.
+__device__ __forceinline__ int worker_of(int total, int w, int n) {
+    int i = min((int)((float)(w + 1) * (float)n / (float)total), n - 1);
+    while (i > 0 && stretch(total, i, n) > w) i--;
+    while (i + 1 < n && stretch(total, i + 1, n) <= w) i++;
+    return i;
+}
 
 struct Request {
-    int start, count, length, blocks, tiles;
+    int start, count, length, old;               // first token, tokens, rows, rows ahead of the pass's (as the lengths say, whatever the table holds)
+    int blocks, tiles;
 };
 __device__ __forceinline__ Request request_of(const PagedParams& p, int b) {
     Request r;
@@ -88,46 +100,41 @@ __device__ __forceinline__ Request request_of(const PagedParams& p, int b) {
     r.start = min(max(s0, 0), p.tokens);
     r.count = min(max(s1 - r.start, 0), p.tokens - r.start);
     r.length = (int)min((long long)max(len, 0), (long long)p.table_width * p.page_size);
+    r.old = len - (s1 - s0);
     r.blocks = (r.length + kKeys - 1) / kKeys;
     r.tiles = (r.count + p.tile_tokens - 1) / p.tile_tokens * p.head_sets;
     return r;
 }
 
-struct Piece {
+// A worker's place in the line: block kb of `blocks` of a segment.
+struct Cursor {
+    int w, end;                                  // in the line
+    int kb, blocks;
     int req;                                     // -1: the prefix
-    int tok0, toks, hs, hk;
-    int kb0, kb1, length;
-    int old;                                     // rows ahead of the pass's (own segments)
+    int hk, tile;
+    Request r;                                   // of the prefix: all tokens, its rows
+    __device__ __forceinline__ int last() const { return min(blocks, kb + end - w); }      // where its piece of the segment ends
 };
-// The piece of block w of the line of single streams, up to `end`; cum: own blocks ahead of each request.
-__device__ __forceinline__ void tile_tokens(const PagedParams& p, int tile, int start, int count, Piece& c) {
-    const int ts = tile / p.head_sets;
-    c.hs = tile - ts * p.head_sets;
-    c.tok0 = start + ts * p.tile_tokens;
-    c.toks = min(p.tile_tokens, count - ts * p.tile_tokens);
+__device__ __forceinline__ void enter(Cursor& c, const Request* reqs, int req) {
+    c.req = req;
+    c.r = reqs[req];
+    c.blocks = c.r.blocks;
+    c.tile = c.hk = c.kb = 0;
 }
-__device__ __forceinline__ Piece piece_of_pair(const PagedParams& p, const Line& l, int w, int end, int s) {
-    Piece c;
-    const int seg = w / l.nbp;
-    c.req = -1;
-    c.kb0 = w - seg * l.nbp;
-    c.kb1 = min(l.nbp, c.kb0 + end - w);
-    c.hk = seg / l.pairs;
-    c.length = p.prefix;
-    c.old = p.prefix;
-    tile_tokens(p, 2 * (seg - c.hk * l.pairs) + s, 0, p.tokens, c);
-    return c;
-}
-__device__ __forceinline__ Piece piece_of(const PagedParams& p, const Line& l, const int* cum, int w, int end) {
-    Piece c;
-    if (w < l.odd) {
+// The cursor of block w of the line of pairs (its tile is the first stream's) or of single streams; cum: own blocks ahead of each request.
+__device__ __forceinline__ Cursor cursor_at(const PagedParams& p, const Line& l, const int* cum, const Request* reqs, bool pair, int w, int end) {
+    Cursor c{};
+    c.w = w;
+    c.end = end;
+    if (w >= end) return c;
+    if (pair || w < l.odd) {
+        const int seg = w / l.nbp;
         c.req = -1;
-        c.hk = w / l.nbp;
-        c.kb0 = w - c.hk * l.nbp;
-        c.kb1 = min(l.nbp, c.kb0 + end - w);
-        c.length = p.prefix;
-        c.old = p.prefix;
-        tile_tokens(p, l.tiles - 1, 0, p.tokens, c);
+        c.r = {0, p.tokens, p.prefix, p.prefix, l.nbp, l.tiles};
+        c.blocks = l.nbp;
+        c.kb = w - seg * l.nbp;
+        c.hk = pair ? seg / l.pairs : seg;
+        c.tile = pair ? 2 * (seg - c.hk * l.pairs) : l.tiles - 1;
         return c;
     }
     const int v = w - l.odd;
@@ -137,16 +144,45 @@ __device__ __forceinline__ Piece piece_of(const PagedParams& p, const Line& l, c
         if (cum[mid] <= v) lo = mid;
         else hi = mid;
     }
-    const Request r = request_of(p, lo);
-    const int in = v - cum[lo], seg = in / r.blocks, tile = seg / p.kv_heads;
-    c.req = lo;
-    c.hk = seg - tile * p.kv_heads;
-    c.kb0 = in - seg * r.blocks;
-    c.kb1 = min(r.blocks, c.kb0 + end - w);
-    c.length = r.length;
-    c.old = p.lengths[lo] - (p.row_starts[lo + 1] - p.row_starts[lo]);
-    tile_tokens(p, tile, r.start, r.count, c);
+    enter(c, reqs, lo);
+    const int in = v - cum[lo], seg = in / c.blocks;
+    c.kb = in - seg * c.blocks;
+    c.tile = seg / p.kv_heads;
+    c.hk = seg - c.tile * p.kv_heads;
     return c;
+}
+// Past its piece.
+__device__ __forceinline__ void advance(Cursor& c, const PagedParams& p, const Line& l, const Request* reqs, bool pair) {
+    const int n = c.last() - c.kb;
+    c.w += n;
+    c.kb += n;
+    if (c.kb < c.blocks || c.w >= c.end) return;
+    c.kb = 0;
+    if (pair) {
+        c.tile += 2;
+        if (c.tile < 2 * l.pairs) return;
+        c.tile = 0;
+        c.hk++;
+        return;
+    }
+    if (++c.hk < p.kv_heads) return;
+    c.hk = 0;
+    if (c.req >= 0 && ++c.tile < c.r.tiles) return;
+    int b = c.req + 1;
+    while (b + 1 < p.requests && reqs[b].blocks * reqs[b].tiles == 0) b++;
+    enter(c, reqs, b);
+}
+// The tile's tokens and heads.
+struct Tile {
+    int tok0, toks, hs;
+};
+__device__ __forceinline__ Tile tile_of(const PagedParams& p, const Request& r, int tile) {
+    Tile x;
+    const int ts = p.head_sets == 1 ? tile : tile / p.head_sets;
+    x.hs = tile - ts * p.head_sets;
+    x.tok0 = r.start + ts * p.tile_tokens;
+    x.toks = min(p.tile_tokens, r.count - ts * p.tile_tokens);
+    return x;
 }
 
 __device__ __forceinline__ uint64_t sw128_desc_n_major(uint32_t saddr, uint32_t box) {      // V: keys by dims, the next 64 dims `box` bytes on
@@ -181,14 +217,33 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
                  "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
                  "r"(r[31]) : "memory");
 }
-__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
-                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+                 "r"(r[14]), "r"(r[15]) : "memory");
 }
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half*) { return h2_as_u32(__floats2half2_rn(lo, hi)); }
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16*) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A value that is the same in all lanes, as one that the compiler knows to be: operands of products and copies then stay in uniform registers.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
+// Two fp32 values at a time (an instruction of half the issue slots).
+__device__ __forceinline__ void fma2(float& x, float& y, float m, float c) {
+    asm("{\n\t.reg .b64 a, m, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 m, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\tfma.rn.f32x2 a, a, m, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(x), "+f"(y) : "f"(m), "f"(c));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float u, float v) {
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(x), "+f"(y) : "f"(u), "f"(v));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 template <typename T, int HD>
@@ -197,12 +252,15 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
     constexpr int ST = G::SLOTS, NB = HD / 64;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
-    __shared__ uint64_t full[ST], freed[ST], qfull[2], qfree[2], sfull[2], pready[2], pvdone[2];
+    __shared__ uint64_t kfull[ST], kfree[ST], vfull[ST], vfree[ST], qfull[2][2], qfree[2][2], sfull[2], pready[2], pvdone[2];
     __shared__ uint32_t s_tmem;
     __shared__ int s_cum[kPgMaxRequests + 1];
-    __shared__ long long s_warp[kPgThreads / 32], s_total;
+    __shared__ Request s_req[kPgMaxRequests];
+    __shared__ long long s_warp[kPgThreads / 32];
+    __shared__ Cursor s_from[3];                                         // of the pairs, of either stream
+    __shared__ float s_part[2][2][kParts][kRows];                        // [stream][in turn]: what a row's threads tell one another
     const uint32_t sbase = smem_u32(smem);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ctas = gridDim.x, cta = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = uniform(threadIdx.x >> 5), ctas = gridDim.x, cta = blockIdx.x;
 
     if (threadIdx.x == 0) {
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(&p.kmap) : "memory");
@@ -210,14 +268,18 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(&p.qmap) : "memory");
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(&p.q1map) : "memory");
         for (int s = 0; s < ST; s++) {
-            mbar_init(smem_u32(full + s), 1);
-            mbar_init(smem_u32(freed + s), 1);
+            mbar_init(smem_u32(kfull + s), 1);
+            mbar_init(smem_u32(kfree + s), 1);
+            mbar_init(smem_u32(vfull + s), 1);
+            mbar_init(smem_u32(vfree + s), 1);
         }
         for (int s = 0; s < 2; s++) {
-            mbar_init(smem_u32(qfull + s), 1);
-            mbar_init(smem_u32(qfree + s), 1);
+            for (int u = 0; u < 2; u++) {
+                mbar_init(smem_u32(&qfull[s][u]), 1);
+                mbar_init(smem_u32(&qfree[s][u]), 1);
+            }
             mbar_init(smem_u32(sfull + s), 1);
-            mbar_init(smem_u32(pready + s), 4);
+            mbar_init(smem_u32(pready + s), 4 * kParts);
             mbar_init(smem_u32(pvdone + s), 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -239,6 +301,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
         long long mine = 0, before;
         for (int b = b0; b < b1; b++) {
             const Request r = request_of(p, b);
+            s_req[b] = r;
             mine += (long long)r.blocks * r.tiles * p.kv_heads;
         }
         long long scan = mine;
@@ -253,144 +316,196 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
         for (int w = 0; w < warp; w++) before += s_warp[w];
         for (int b = b0; b < b1; b++) {
             s_cum[b] = (int)min(before, 1ll << 30);
-            const Request r = request_of(p, b);
-            before += (long long)r.blocks * r.tiles * p.kv_heads;
+            before += (long long)s_req[b].blocks * s_req[b].tiles * p.kv_heads;
         }
-        if (threadIdx.x == kPgThreads - 1) {
-            s_cum[p.requests] = (int)min(before, 1ll << 30);
-            s_total = s_cum[p.requests];
-        }
+        if (threadIdx.x == kPgThreads - 1) s_cum[p.requests] = (int)min(before, 1ll << 30);
         __syncthreads();
     }
-    if (cta == 0)
-        for (int b = threadIdx.x; b <= p.requests; b += kPgThreads) p.plan[b] = s_cum[b];
-    const Line l = line_of(p, s_total);
-    // This CTA's stretch of the pairs, and its streams' of the rest.
-    const int a0 = (int)stretch(l.pair_total, cta, ctas), a1 = (int)stretch(l.pair_total, cta + 1, ctas);
-    const int w0 = (int)stretch(l.total, 2 * cta, 2 * ctas), w1 = (int)stretch(l.total, 2 * cta + 1, 2 * ctas), w2 = (int)stretch(l.total, 2 * cta + 2, 2 * ctas);
-    const int from[2] = {w0, w1}, to[2] = {w1, w2};
+    const Line l = line_of(p, s_cum[p.requests]);
+    // This CTA's stretch of the pairs, and its streams' of the rest.  Every other CTA begins with the rest: pairs keep the tensor cores busy, the
+    // rest the memory.
+    const int turn = cta & 1;
+    if (threadIdx.x < 3) {
+        const bool pair = threadIdx.x == 0;
+        const int total = pair ? l.pair_total : l.total, i = pair ? cta : 2 * cta + threadIdx.x - 1, n = pair ? ctas : 2 * ctas;
+        s_from[threadIdx.x] = cursor_at(p, l, s_cum, s_req, pair, stretch(total, i, n), stretch(total, i + 1, n));
+    } else if (cta == 0 && warp > 0) {
+        for (int b = threadIdx.x - 32; b <= p.requests; b += kPgThreads - 32) p.plan[b] = s_cum[b];
+    }
+    __syncthreads();
+    const int np = uniform(s_from[0].end - s_from[0].w), n0 = uniform(s_from[1].end - s_from[1].w), n1 = uniform(s_from[2].end - s_from[2].w);
 
-    if (warp == kLoader) {
-        // ------------------------------------------------------------------ keys and values, in the order of their use
+    if (warp == kKeyLoader || warp == kValueLoader) {
+        // ------------------------------------------------------------------ keys and queries, or values, in the order of their use
         asm volatile("fence.proxy.async;\n" ::: "memory");               // (appended by ordinary stores of an earlier kernel)
+        const bool values = warp == kValueLoader;
+        const CUtensorMap* map = values ? &p.vmap : &p.kmap;
+        uint64_t *const full = values ? vfull : kfull, *const free = values ? vfree : kfree;
+        const uint32_t slots = sbase + G::KV0 + (values ? ST * G::SLOT : 0);
         int ring = 0;
-        struct At {
-            int w, end, hk, kb, kb1, req, length, page, row, boxes;
-        } at[2];
-        auto open = [&](At& x, const Piece& c) {
-            x.hk = c.hk; x.kb = c.kb0; x.kb1 = c.kb1; x.req = c.req; x.length = c.length;
-        };
-        // pages of the cursor's block: a lane each, or the one that holds all of it
-        auto pages = [&](At& x) {
-            const int key0 = x.kb * kKeys, rows = min(kKeys, x.length - key0);
-            x.boxes = (rows + p.box_rows - 1) / p.box_rows;
-            x.row = p.page_size > kKeys ? key0 % p.page_size : 0;
-            const int index = key0 / p.page_size + lane;
-            if (lane < x.boxes) x.page = x.req < 0 ? p.prefix_pages[index] : p.table[x.req * p.table_stride + index];
-        };
-        auto load = [&](const At& x, const CUtensorMap* map) {
-            const int slot = ring % ST;
-            if (ring >= ST) mbar_wait_reported(smem_u32(freed + slot), (ring / ST - 1) & 1, p.polls, p.err, 31);
-            __syncwarp();
-            const uint32_t bar = smem_u32(full + slot), dst = sbase + G::KV0 + slot * G::SLOT;
-            if (elect_one()) mbar_expect_tx(bar, x.boxes * p.box_rows * HD * 2);
-            __syncwarp();
-            if (lane < x.boxes) {
+        int asked[4] = {0, 0, 0, 0}, half = 3;                           // uses of the streams' halves of queries; the halves last taken, a bit a stream
+        // A tile of queries, or, of 64 rows at most, one of its halves in turn, so that the next piece's come while this one's are in use.
+        auto ask = [&](int s, const Cursor& c, int tile) {
+            const Tile x = tile_of(p, c.r, tile);
+            const int toks = uniform(x.toks), tok0 = uniform(x.tok0), head = uniform(c.hk * p.group + x.hs * p.tile_heads);
+            const bool small = toks * p.tile_heads <= kRows / 2;
+            if (small) half ^= 1 << s;
+            const int u = small ? (half >> s) & 1 : 0;
 #pragma unroll
-                for (int h = 0; h < NB; h++)
-                    tma_box4(dst + h * (kKeys * 128) + lane * p.box_rows * 128, map, h * 64, x.row, x.hk, x.page, bar);
-            }
-            __syncwarp();
-            ring++;
-        };
-        // pairs
-        {
-            At& x = at[0];
-            for (int w = a0; w < a1;) {
-                const Piece c = piece_of_pair(p, l, w, a1, 0);
-                open(x, c);
-                for (; x.kb < x.kb1; x.kb++) {
-                    pages(x);
-                    load(x, &p.kmap);
-                    load(x, &p.vmap);
+            for (int k = 0; k < 4; k++)
+                if (k == 2 * s + u || (!small && k == 2 * s + 1)) {
+                    if (asked[k] > 0) mbar_wait_reported(smem_u32(&qfree[s][k & 1]), (asked[k] - 1) & 1, p.polls, p.err, 31);
+                    asked[k]++;
                 }
-                w += c.kb1 - c.kb0;
+            __syncwarp();
+            if (elect_one()) {
+                const uint32_t bar = smem_u32(&qfull[s][u]), dst = sbase + s * G::QTILE + u * (kRows / 2 * 128);
+                if (small && toks <= 4) {                                // (a box of half the tile would bring 64 rows)
+                    mbar_expect_tx(bar, toks * p.tile_heads * HD * 2);
+                    for (int t = 0; t < toks; t++)
+#pragma unroll
+                        for (int h = 0; h < NB; h++)
+                            tma_box3(dst + h * (kRows * 128) + t * p.tile_heads * 128, &p.q1map, h * 64, head, tok0 + t, bar);
+                } else {
+                    mbar_expect_tx(bar, (small ? p.half_tokens : p.tile_tokens) * p.tile_heads * HD * 2);
+#pragma unroll
+                    for (int h = 0; h < NB; h++) tma_box3(dst + h * (kRows * 128), small ? &p.qhmap : &p.qmap, h * 64, head, tok0, bar);
+                }
             }
-        }
-        // single streams: K a block ahead of V
-        auto next = [&](At& x) {                                         // the cursor's block, its pages
-            if (x.kb == x.kb1) open(x, piece_of(p, l, s_cum, x.w, x.end));
-            pages(x);
-            load(x, &p.kmap);
-            x.w++;
-            x.kb++;
+            __syncwarp();
         };
+        struct At {
+            Cursor c;
+            int kb, kb1;                                                 // of the piece
+            int ahead;                                                   // a page of the next block a lane
+        };
+        auto page_at = [&](const At& x, int kb) {
+            const int key = kb * kKeys + lane * p.box_rows;
+            int page = 0;
+            if (lane * p.box_rows < kKeys && key < x.c.r.length && kb < x.kb1)
+                page = x.c.req < 0 ? p.prefix_pages[key / p.page_size] : p.table[x.c.req * p.table_stride + key / p.page_size];
+            return page;
+        };
+        auto start = [&](At& x, int which) {
+            x.c = s_from[which];
+            x.kb = x.c.kb;
+            x.kb1 = x.c.last();
+            x.ahead = page_at(x, x.kb);
+        };
+        // The cursor's next block; s: the stream that uses it, 2: both.
+        auto next = [&](At& x, int s) {
+            const bool first = x.kb == x.c.kb;
+            const int page = x.ahead, key0 = x.kb * kKeys, row = uniform(p.page_size > kKeys ? key0 % p.page_size : 0), hk = uniform(x.c.hk);
+            const int boxes = uniform((min(kKeys, x.c.r.length - key0) + p.box_rows - 1) / p.box_rows), slot = ring % ST;
+            x.ahead = page_at(x, x.kb + 1);
+            if (ring >= ST) mbar_wait_reported(smem_u32(free + slot), (ring / ST - 1) & 1, p.polls, p.err, 31);
+            __syncwarp();
+            const uint32_t bar = smem_u32(full + slot), dst = slots + slot * G::SLOT;
+            if (elect_one()) mbar_expect_tx(bar, boxes * p.box_rows * HD * 2);
+            __syncwarp();
+#pragma unroll 1
+            for (int j = 0; j < boxes; j++) {
+                const int at = uniform(__shfl_sync(0xffffffffu, page, j));
+                if (elect_one()) {
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-            at[s].w = from[s];
-            at[s].end = to[s];
-            at[s].kb = at[s].kb1 = 0;
-            if (at[s].w < at[s].end) next(at[s]);
-        }
-        for (int i = 0; i < max(w1 - w0, w2 - w1); i++) {
-#pragma unroll
-            for (int s = 0; s < 2; s++) {
-                if (i >= to[s] - from[s]) continue;
-                load(at[s], &p.vmap);
-                if (at[s].w < at[s].end) next(at[s]);
+                    for (int h = 0; h < NB; h++) tma_box4(dst + h * (kKeys * 128) + j * p.box_rows * 128, map, h * 64, row, hk, at, bar);
+                }
+                __syncwarp();
+            }
+            ring++;
+            if (first && !values) {                                      // (behind the keys: their slot is free earlier)
+                if (s != 1) ask(0, x.c, x.c.tile);
+                if (s != 0) ask(1, x.c, x.c.tile + (s == 2));
+            }
+            if (++x.kb == x.kb1) {
+                advance(x.c, p, l, s_req, s == 2);
+                x.kb = x.c.kb;
+                x.kb1 = x.c.last();
+                x.ahead = page_at(x, x.kb);
+            }
+        };
+#pragma unroll 1
+        for (int phase = 0; phase < 2; phase++) {
+            At x, y;
+            if (phase == turn) {
+                if (np > 0) start(x, 0);
+#pragma unroll 1
+                for (int i = 0; i < np; i++) next(x, 2);
+            } else {
+                if (n0 > 0) start(x, 1);
+                if (n1 > 0) start(y, 2);
+#pragma unroll 1
+                for (int i = 0; i < max(n0, n1); i++) {
+                    if (i < n0) next(x, 0);
+                    if (i < n1) next(y, 1);
+                }
             }
         }
     } else if (warp == kIssuer) {
         // ------------------------------------------------------------------ products
         constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
         constexpr uint32_t base = (1u << 4) | ((uint32_t)(kRows >> 4) << 24) | (BF ? (1u << 7) | (1u << 10) : 0u);
-        constexpr uint32_t idesc_o = base | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
-        const uint64_t qdesc = sw128_desc(sbase), kdesc = sw128_desc(sbase + G::KV0), vdesc = sw128_desc_n_major(sbase + G::KV0, kKeys * 128);
-        int ring = 0;
-        int blocks[2] = {0, 0}, pieces[2] = {0, 0};                      // scores asked for, pieces begun
+        constexpr uint32_t idesc_s = base | ((uint32_t)(kKeys >> 3) << 17), idesc_o = base | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
+        const uint64_t qdesc = sw128_desc(sbase), kdesc = sw128_desc(sbase + G::KV0), vdesc = sw128_desc_n_major(sbase + G::KV0 + ST * G::SLOT, kKeys * 128);
         struct At {
-            int w, end, kb, kb1, length;
+            Cursor c;
+            int left;                                                    // blocks of the phase whose scores have not been asked for
+            int kb, kb1;                                                 // of the piece
             int keys;                                                    // of the block whose scores were asked for last
-            bool first, last;                                            // ... of its piece
+            bool first, small;                                           // ... of its piece; its queries take half a tile
+            int blocks, came0, came1, half;                              // scores asked for; arrivals of queries, the half last used
         } at[2];
-        // Scores of the cursor's block of stream s.
-        auto scores = [&](int s, At& x, bool take, bool give) {
-            const int slot = ring % ST;
-            if (take) {
-                mbar_wait_reported(smem_u32(full + slot), (ring / ST) & 1, p.polls, p.err, 31);
-            }
+        int kring = 0, vring = 0;
+        // Scores of the next block of stream s.  take: wait for its keys, give: hand them back (a pair's second stream does).
+        auto scores = [&](int s, At& x, bool pair, bool take, bool give) {
+            const int slot = kring % ST;
+            x.first = x.kb == x.kb1;
             if (x.first) {
-                mbar_wait_reported(smem_u32(qfull + s), pieces[s] & 1, p.polls, p.err, 31);
-                pieces[s]++;
+                x.kb = uniform(x.c.kb);
+                x.kb1 = uniform(x.c.last());
+                x.small = uniform(tile_of(p, x.c.r, x.c.tile + (pair ? s : 0)).toks) * p.tile_heads <= kRows / 2;
+                if (x.small) x.half ^= 1;
+                const int q = x.small ? x.half : 0;
+                mbar_wait_reported(smem_u32(&qfull[s][q]), (q ? x.came1 : x.came0) & 1, p.polls, p.err, 31);
+                if (q) x.came1++;
+                else x.came0++;
             }
-            if (blocks[s] > 0) mbar_wait_reported(smem_u32(pvdone + s), (blocks[s] - 1) & 1, p.polls, p.err, 31);      // (probabilities where the scores go)
+            x.keys = uniform(min(kKeys, x.c.r.length - x.kb * kKeys));
+            x.kb++;
+            x.left--;
+            const bool last = x.kb == x.kb1;
+            if (take) mbar_wait_reported(smem_u32(kfull + slot), (kring / ST) & 1, p.polls, p.err, 31);
+            if (x.blocks > 0) mbar_wait_reported(smem_u32(pvdone + s), (x.blocks - 1) & 1, p.polls, p.err, 31);      // (probabilities stand where the scores go)
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             __syncwarp();
             if (elect_one()) {
-                const uint32_t d = tmem + s * kKeys, idesc = base | ((uint32_t)((x.keys + 15) / 16 * 2) << 17);
-                const uint64_t q0 = qdesc + s * (G::QTILE / 16), k0 = kdesc + slot * (G::SLOT / 16);
+                const int q = x.small ? x.half : 0;
+                const uint64_t q0 = qdesc + s * (G::QTILE / 16) + q * (kRows / 2 * 128 / 16), k0 = kdesc + slot * (G::SLOT / 16);
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ks++)
-                    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-                                 "l"(q0 + (ks >> 2) * (kRows * 128 / 16) + (ks & 3) * 2), "l"(k0 + (ks >> 2) * (kKeys * 128 / 16) + (ks & 3) * 2), "r"(idesc),
+                    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem + s * kKeys),
+                                 "l"(q0 + (ks >> 2) * (kRows * 128 / 16) + (ks & 3) * 2), "l"(k0 + (ks >> 2) * (kKeys * 128 / 16) + (ks & 3) * 2), "r"(idesc_s),
                                  "r"(ks) : "memory");
                 commit_to(smem_u32(sfull + s));
-                if (give) commit_to(smem_u32(freed + slot));
-                if (x.last) commit_to(smem_u32(qfree + s));
+                if (give) commit_to(smem_u32(kfree + slot));
+                if (last) {
+                    commit_to(smem_u32(&qfree[s][q]));
+                    if (!x.small) commit_to(smem_u32(&qfree[s][1]));
+                }
             }
             __syncwarp();
-            blocks[s]++;
-            if (give) ring++;
+            x.blocks++;
+            if (give) kring++;
+            if (last) advance(x.c, p, l, s_req, pair);
         };
         // Output of the block whose scores stream s asked for last.
         auto output = [&](int s, const At& x, bool take, bool give) {
-            const int slot = ring % ST;
-            const int steps = (x.keys + 15) / 16;
+            const int slot = vring % ST, steps = (x.keys + 15) / 16;
             if (take) {
-                mbar_wait_reported(smem_u32(full + slot), (ring / ST) & 1, p.polls, p.err, 31);
+                mbar_wait_reported(smem_u32(vfull + slot), (vring / ST) & 1, p.polls, p.err, 31);
                 if (x.keys & 15) {
                     // Rows behind the last, up to the step of the product: whatever is there has probability 0, and 0 x Inf or NaN would be NaN.
-                    const uint32_t v = sbase + G::KV0 + slot * G::SLOT;
+                    const uint32_t v = sbase + G::KV0 + (ST + slot) * G::SLOT;
                     for (int k = x.keys * 8 + lane; k < steps * 16 * 8; k += 32)
 #pragma unroll
                         for (int h = 0; h < NB; h++)
@@ -399,214 +514,156 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
                     __syncwarp();
                 }
             }
-            mbar_wait_reported(smem_u32(pready + s), (blocks[s] - 1) & 1, p.polls, p.err, 31);
+            mbar_wait_reported(smem_u32(pready + s), (x.blocks - 1) & 1, p.polls, p.err, 31);
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             __syncwarp();
             if (elect_one()) {
                 const uint64_t v0 = vdesc + slot * (G::SLOT / 16);
-                const uint32_t d = tmem + 2 * kKeys + s * HD, a0 = tmem + s * kKeys;
-                for (int ks = 0; ks < steps; ks++)
-                    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-                                 "r"(a0 + ks * 8), "l"(v0 + ks * (2048 / 16)), "r"(idesc_o), "r"((x.first ? 0 : 1) + ks) : "memory");
-                if (give) commit_to(smem_u32(freed + slot));
+#pragma unroll
+                for (int ks = 0; ks < kKeys / 16; ks++)                  // (each part's probabilities stand at the beginning of its scores)
+                    if (ks < steps)
+                        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem + 2 * kKeys + s * HD),
+                                     "r"(tmem + s * kKeys + ks / 4 * (kKeys / kParts) + ks % 4 * 8), "l"(v0 + ks * (2048 / 16)), "r"(idesc_o),
+                                     "r"((x.first ? 0 : 1) + ks) : "memory");
+                if (give) commit_to(smem_u32(vfree + slot));
                 commit_to(smem_u32(pvdone + s));                         // (the last thing that a CTA's end waits for)
             }
             __syncwarp();
-            if (give) ring++;
+            if (give) vring++;
         };
-        auto enter = [&](At& x) {
-            x.first = x.kb == x.kb1;
-        };
-        auto block = [&](At& x, int kb) {                                // the cursor stands before block kb
-            x.keys = min(kKeys, x.length - kb * kKeys);
-            x.last = kb + 1 == x.kb1;
-            x.kb = kb + 1;
-            x.w++;
-        };
-        auto pair_next = [&](At& x) {
-            enter(x);
-            if (x.first) {
-                const Piece c = piece_of_pair(p, l, x.w, a1, 0);
-                x.kb = c.kb0;
-                x.kb1 = c.kb1;
-                x.length = c.length;
-            }
-            block(x, x.kb);
-        };
-        auto next = [&](At& x) {
-            enter(x);
-            if (x.first) {
-                const Piece c = piece_of(p, l, s_cum, x.w, x.end);
-                x.kb = c.kb0;
-                x.kb1 = c.kb1;
-                x.length = c.length;
-            }
-            block(x, x.kb);
-        };
-        if (a0 < a1) {
-            At x, y;                                                     // the block whose output is next; the one whose scores are
-            x.w = a0;
-            x.kb = x.kb1 = 0;
-            pair_next(x);
-            scores(0, x, true, false);
-            scores(1, x, false, true);
-            for (int i = a0; i < a1; i++) {
-                // (V of this block stands ahead of the next block's K in the ring: `ring` is V's)
-                y = x;
-                const bool more = i + 1 < a1;
-                if (more) pair_next(y);
-                output(0, x, true, false);
-                if (more) {
-                    ring++;
-                    scores(0, y, true, false);
-                    ring--;
-                }
-                output(1, x, false, true);
-                if (more) scores(1, y, false, true);
-                x = y;
-            }
-        }
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            at[s].w = from[s];
-            at[s].end = to[s];
-            at[s].kb = at[s].kb1 = 0;
-            if (at[s].w < at[s].end) {
-                next(at[s]);
-                scores(s, at[s], true, true);
-            }
+            at[s].blocks = at[s].came0 = at[s].came1 = 0;
+            at[s].half = 1;
         }
-        for (int i = 0; i < max(w1 - w0, w2 - w1); i++) {
+#pragma unroll 1
+        for (int phase = 0; phase < 2; phase++) {
+            const bool pair = phase == turn;
 #pragma unroll
             for (int s = 0; s < 2; s++) {
-                if (i >= to[s] - from[s]) continue;
-                output(s, at[s], true, true);
-                if (at[s].w < at[s].end) {
-                    next(at[s]);
-                    scores(s, at[s], true, true);
-                }
+                at[s].c = s_from[pair ? 0 : 1 + s];
+                at[s].left = pair ? np : (s ? n1 : n0);
+                at[s].kb = at[s].kb1 = 0;
             }
-        }
-    } else if (warp >= kQueries) {
-        // ------------------------------------------------------------------ queries of stream s, a piece ahead of nobody: once the last piece's scores are done
-        asm volatile("fence.proxy.async;\n" ::: "memory");
-        const int s = warp - kQueries;
-        int piece = 0;
-        auto load = [&](const Piece& c) {
-            if (piece > 0) mbar_wait_reported(smem_u32(qfree + s), (piece - 1) & 1, p.polls, p.err, 31);
-            __syncwarp();
-            if (elect_one()) {
-                const uint32_t bar = smem_u32(qfull + s), dst = sbase + s * G::QTILE;
-                const int head = c.hk * p.group + c.hs * p.tile_heads;
-                if (c.toks <= 4) {                                       // (a box of the whole tile would bring 128 rows)
-                    mbar_expect_tx(bar, c.toks * p.tile_heads * HD * 2);
-                    for (int t = 0; t < c.toks; t++)
 #pragma unroll
-                        for (int h = 0; h < NB; h++)
-                            tma_box3(dst + h * (kRows * 128) + t * p.tile_heads * 128, &p.q1map, h * 64, head, c.tok0 + t, bar);
-                } else {
-                    mbar_expect_tx(bar, p.tile_tokens * p.tile_heads * HD * 2);
+            for (int s = 0; s < 2; s++)
+                if (at[s].left > 0) scores(s, at[s], pair, !pair || s == 0, !pair || s == 1);
+            const int most = pair ? np : max(n0, n1);
+#pragma unroll 1
+            for (int i = 0; i < most; i++)
 #pragma unroll
-                    for (int h = 0; h < NB; h++) tma_box3(dst + h * (kRows * 128), &p.qmap, h * 64, head, c.tok0, bar);
+                for (int s = 0; s < 2; s++) {
+                    if (i >= (pair ? np : (s ? n1 : n0))) continue;
+                    output(s, at[s], !pair || s == 0, !pair || s == 1);
+                    if (at[s].left > 0) scores(s, at[s], pair, !pair || s == 0, !pair || s == 1);
                 }
-            }
-            __syncwarp();
-            piece++;
-        };
-        for (int w = a0; w < a1;) {
-            const Piece c = piece_of_pair(p, l, w, a1, s);
-            load(c);
-            w += c.kb1 - c.kb0;
         }
-        for (int w = from[s]; w < to[s];) {
-            const Piece c = piece_of(p, l, s_cum, w, to[s]);
-            load(c);
-            w += c.kb1 - c.kb0;
-        }
-    } else {
-        // ------------------------------------------------------------------ softmax: a query row a thread
-        const int s = warp >> 2, r = (warp & 3) * 32 + lane;
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tS = tmem + s * kKeys + lanes, tO = tmem + 2 * kKeys + s * HD + lanes;
+    } else if (warp < kKeyLoader) {
+        // ------------------------------------------------------------------ softmax: 64 keys of a block of a query row a thread
+        constexpr int KEYS = kKeys / kParts, HALF = KEYS / 2, DIMS = HD / kParts;
+        const int s = warp >> 3, part = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tS = tmem + s * kKeys + part * KEYS + lanes, tO = tmem + 2 * kKeys + s * HD + part * DIMS + lanes;
         const int dt = r / p.tile_heads;
+        auto row_sync = [&]() { asm volatile("bar.sync %0, %1;\n" ::"r"(1 + s * 4 + (warp & 3)), "n"(kParts * 32) : "memory"); };      // the warps of these rows
         int blocks = 0;
-        auto run = [&](const Piece& c, bool pair, int worker) {
-            const int rows = c.toks * p.tile_heads, g = c.hs * p.tile_heads + r - dt * p.tile_heads, t = c.tok0 + dt;
-            const bool valid = dt < c.toks && g < p.group, busy = (warp & 3) * 32 < rows;      // (busy: some row of the warp may be)
+        auto run = [&](const Cursor& c, bool pair) {
+            const Tile tile = tile_of(p, c.r, c.tile + (pair ? s : 0));
+            const int rows = tile.toks * p.tile_heads, g = tile.hs * p.tile_heads + r - dt * p.tile_heads, t = tile.tok0 + dt, kb1 = c.last();
+            const bool valid = dt < tile.toks && g < p.group, busy = (warp & 3) * 32 < rows;      // (busy: some row of the warp may be)
             // The first key that this row does not see by its place; the new rows it sees by mask.
             const bool masked = c.req >= 0 && p.mask != nullptr;
-            int limit = c.length;
+            const int length = c.r.length, old = c.r.old, sure = min(old, length);      // (sure: keys up to here are seen by all rows)
+            int limit = length;
             unsigned long long bits = 0;
             if (c.req >= 0) {
-                limit = min(limit, masked ? c.old : c.old + (t - p.row_starts[c.req]) + 1);
+                limit = min(limit, masked ? old : old + (t - c.r.start) + 1);
                 if (masked && valid) bits = p.mask[t];
             }
-            const int sure = c.req < 0 ? c.length : c.old;               // keys up to here are seen by all rows
-            float m = -INFINITY, sum = 0.f;
+            float m = -INFINITY, sum[2] = {0.f, 0.f};                    // the reference of the row's weights, no more than 2^kLag below its maximum
 #pragma unroll 1
-            for (int kb = c.kb0; kb < c.kb1; kb++, blocks++) {
+            for (int kb = c.kb; kb < kb1; kb++, blocks++) {
                 mbar_wait_reported(smem_u32(sfull + s), blocks & 1, p.polls, p.err, 31);
                 __syncwarp();
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                 if (busy) {
-                    uint32_t raw[kKeys];
+                    const int key0 = kb * kKeys + part * KEYS;
+                    // Half of the scores at a time; what the row does not see is minus infinity.
+                    float a[HALF];
+                    auto scores = [&](int h) {
+                        uint32_t raw[HALF];
+                        tmem_ld32(raw, tS + h * HALF);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
-                    for (int j = 0; j < kKeys; j += 32) tmem_ld32(raw + j, tS + j);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-                    const int key0 = kb * kKeys;
-                    if (p.negative) {
+                        for (int j = 0; j < HALF; j++) a[j] = __uint_as_float(raw[j]);
+                        if (p.negative) {
 #pragma unroll
-                        for (int j = 0; j < kKeys; j++) raw[j] ^= 0x80000000u;
-                    }
-                    if (key0 + kKeys > sure || key0 + kKeys > c.length) {
-#pragma unroll
-                        for (int w = 0; w < kKeys / 32; w++) {
-                            const int n = limit - key0 - 32 * w, o = key0 + 32 * w - c.old;      // keys of the word ahead of the limit; first key's new row
-                            uint32_t seen = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
-                            if (masked && o > -32 && o < 64) {
-                                uint32_t x = (uint32_t)(o >= 0 ? bits >> o : bits << -o);
-                                const int there = c.length - key0 - 32 * w;
-                                if (there < 32) x &= there <= 0 ? 0u : (1u << there) - 1u;
-                                seen |= x;
-                            }
-#pragma unroll
-                            for (int j = 0; j < 32; j++)
-                                if (!((seen >> j) & 1u)) raw[32 * w + j] = 0xff800000u;
+                            for (int j = 0; j < HALF; j++) a[j] = -a[j];
                         }
-                    }
-                    float x[4];
+                        const int k0 = key0 + h * HALF;
+                        if (k0 + HALF > sure) {
+                            const int o = k0 - old, there = length - k0, n = limit - k0;      // the first key among the new rows; keys there are; keys seen
+                            uint32_t seen = n >= HALF ? ~0u : (n <= 0 ? 0u : (1u << n) - 1);
+                            if (masked && o > -HALF && o < 64) seen |= (uint32_t)(o >= 0 ? bits >> o : bits << -o) & (there >= HALF ? ~0u : (there <= 0 ? 0u : (1u << there) - 1));
 #pragma unroll
-                    for (int j = 0; j < 4; j++) x[j] = fmaxf(__uint_as_float(raw[j]), __uint_as_float(raw[4 + j]));
+                            for (int j = 0; j < HALF; j++)
+                                if (!((seen >> j) & 1)) a[j] = -INFINITY;
+                        }
+                    };
+                    float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    auto highest = [&]() {
 #pragma unroll
-                    for (int j = 8; j < kKeys; j++) x[j & 3] = fmaxf(x[j & 3], __uint_as_float(raw[j]));
-                    const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * p.scale_log2;
-                    const bool grown = top > m;
+                        for (int j = 0; j < HALF; j += 8) {
+#pragma unroll
+                            for (int e = 0; e < 4; e++) x[e] = max3(x[e], a[j + e], a[j + 4 + e]);
+                        }
+                    };
+                    scores(0);
+                    highest();
+                    scores(1);
+                    highest();
+                    float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * p.scale_log2;
+                    s_part[s][blocks & 1][part][r] = top;
+                    row_sync();
+                    top = fmaxf(top, s_part[s][blocks & 1][part ^ 1][r]);
+                    const bool grown = top > m + kLag;                   // (of no key so far: m is minus infinity)
                     const float al = !grown ? 1.f : (m == -INFINITY ? 0.f : exp2_approx(m - top));
                     if (grown) m = top;
                     const float ref = m == -INFINITY ? 0.f : -m;
-                    if (__any_sync(0xffffffffu, grown && valid) && kb > c.kb0) {
+                    const bool rescale = __any_sync(0xffffffffu, grown && valid) && kb > c.kb;      // (the same in the rows' other warp)
+                    float more[4] = {0.f, 0.f, 0.f, 0.f};
+                    auto weights = [&](int h) {                          // -> the beginning of the scores, which have been read
+                        uint32_t pk[HALF / 2];
+#pragma unroll
+                        for (int j = 0; j < HALF; j += 2) {
+                            float e0 = a[j], e1 = a[j + 1];
+                            fma2(e0, e1, p.scale_log2, ref);
+                            e0 = exp2_approx(e0);
+                            e1 = exp2_approx(e1);
+                            add2(more[j & 2], more[(j & 2) + 1], e0, e1);
+                            pk[j / 2] = pack2(e0, e1, (T*)nullptr);
+                        }
+                        tmem_st16(tS + h * (HALF / 2), pk);
+                    };
+                    // (read again: 64 more registers are not there.  The second half's weights go behind the first's, 16 to 31 of the 64 columns: its own
+                    // scores begin at 32)
+                    scores(0);
+                    weights(0);
+                    scores(1);
+                    weights(1);
+                    sum[0] = sum[0] * al + (more[0] + more[2]);
+                    sum[1] = sum[1] * al + (more[1] + more[3]);
+                    if (rescale) {
                         // (the block before has been added: its product was waited for ahead of these scores)
 #pragma unroll
-                        for (int d = 0; d < HD; d += 16) {               // (few at a time: the scores stand in 128 registers)
-                            uint32_t o[16];
-                            tmem_ld<16>(o, tO + d);
+                        for (int d = 0; d < DIMS; d += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(o, tO + d);
                             asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
-                            for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * al);
-                            tmem_st8(tO + d, o);
-                            tmem_st8(tO + d + 8, o + 8);
+                            for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * al);
+                            tmem_st32(tO + d, o);
                         }
                     }
-                    float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int j = 0; j < kKeys; j += 2) {
-                        const float e0 = exp2_approx(fmaf(__uint_as_float(raw[j]), p.scale_log2, ref)), e1 = exp2_approx(fmaf(__uint_as_float(raw[j + 1]), p.scale_log2, ref));
-                        part[j & 2] += e0;
-                        part[(j & 2) + 1] += e1;
-                        raw[j / 2] = pack2(e0, e1, (T*)nullptr);
-                    }
-                    tmem_st32(tS, raw);
-                    tmem_st32(tS + 32, raw + 32);
-                    sum = sum * al + ((part[0] + part[1]) + (part[2] + part[3]));
                     asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
@@ -618,42 +675,47 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
             __syncwarp();
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             if (busy) {
+                float l = sum[0] + sum[1];
+                s_part[s][blocks & 1][part][r] = l;                      // (not where the last block's maximum was)
+                row_sync();
+                l += s_part[s][blocks & 1][part ^ 1][r];
                 const long long row = (long long)t * p.heads + c.hk * p.group + g, all = (long long)p.tokens * p.heads;
                 float* dst;
                 long long at;
-                if (c.kb0 == 0) {
+                if (c.kb == 0) {
                     dst = (c.req < 0 ? p.first_prefix : p.first_own) + row * HD;
                     at = (c.req < 0 ? 0 : all) + row;
-                } else if (pair) {
-                    dst = p.more_pair + ((long long)worker * 2 * kRows + s * kRows + r) * HD;
-                    at = 2 * all + (long long)worker * 2 * kRows + s * kRows + r;
                 } else {
-                    dst = p.more + ((long long)worker * kRows + r) * HD;
-                    at = 2 * all + (long long)ctas * 2 * kRows + (long long)worker * kRows + r;
+                    // (pairs: 256 rows a CTA; single streams: 128 a stream, behind them)
+                    const long long slot = (long long)cta * 2 * kRows + s * kRows + r;
+                    dst = (pair ? p.more_pair : p.more) + slot * HD;
+                    at = 2 * all + (pair ? 0 : (long long)ctas * 2 * kRows) + slot;
                 }
-                if (valid) p.ml[at] = make_float2(m, sum);
+                if (valid && part == 0) p.ml[at] = make_float2(l == l ? m : INFINITY, l);      // (scores of NaN alone leave no maximum, but the row is NaN)
 #pragma unroll
-                for (int d = 0; d < HD; d += 32) {
+                for (int d = 0; d < DIMS; d += 32) {
                     uint32_t o[32];
                     tmem_ld32(o, tO + d);
                     asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
                     if (valid) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(dst + d + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        for (int j = 0; j < 32; j += 8)                  // (whole sectors: halves of them took twice as long)
+                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(dst + part * DIMS + d + j), "r"(o[j]), "r"(o[j + 1]),
+                                         "r"(o[j + 2]), "r"(o[j + 3]), "r"(o[j + 4]), "r"(o[j + 5]), "r"(o[j + 6]), "r"(o[j + 7]) : "memory");
                     }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
             }
         };
-        for (int w = a0; w < a1;) {
-            const Piece c = piece_of_pair(p, l, w, a1, s);
-            run(c, true, cta);
-            w += c.kb1 - c.kb0;
-        }
-        for (int w = from[s]; w < to[s];) {
-            const Piece c = piece_of(p, l, s_cum, w, to[s]);
-            run(c, false, 2 * cta + s);
-            w += c.kb1 - c.kb0;
+#pragma unroll 1
+        for (int phase = 0; phase < 2; phase++) {
+            const bool pair = phase == turn;
+            Cursor c = s_from[pair ? 0 : 1 + s];
+#pragma unroll 1
+            while (c.w < c.end) {
+                run(c, pair);
+                advance(c, p, l, s_req, pair);
+            }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
@@ -664,12 +726,12 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
     }
 }
 
-// A warp joins the pieces of one query row.  `ctas` is the grid of the kernel above.
+// A warp joins the pieces of one query row: a lane looks at a piece's statistics, then all lanes add its output, four dims (two) each.
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedParams p, int ctas) {
     pdl_launch_dependents();
     pdl_wait();
-    constexpr int N = HD / 32;
+    constexpr int N = HD / 32, BATCH = 4;
     const int lane = threadIdx.x & 31, head = blockIdx.y * 4 + (threadIdx.x >> 5), t = blockIdx.x;
     if (head >= p.heads) return;
     if (t < p.row_starts[0] || t >= p.row_starts[p.requests]) return;
@@ -684,42 +746,109 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     const Line l = line_of(p, p.plan[p.requests]);
     const int hk = head / p.group, g = head - hk * p.group, hs = g / p.tile_heads, in = g - hs * p.tile_heads;
     const long long row = (long long)t * p.heads + head, all = (long long)p.tokens * p.heads;
-    float m = -INFINITY, sum = 0.f, o[N] = {};
-    auto add = [&](const float* src, float2 x) {
-        if (x.x == -INFINITY) return;
-        const float top = fmaxf(m, x.x), a = exp2_approx(m - top), b = exp2_approx(x.x - top);
-        sum = sum * a + x.y * b;
-#pragma unroll
-        for (int e = 0; e < N; e++) o[e] = o[e] * a + src[lane * N + e] * b;
-        m = top;
-    };
-    auto pieces = [&](long long total, long long start, int blocks, int workers, const float* first, long long first_ml, const float* more, long long more_ml,
-                      int rows, int r) {
-        if (blocks == 0) return;
-        add(first + row * HD, p.ml[first_ml + row]);
-        const int last = worker_of(total, start + blocks - 1, workers);
-        for (int w = worker_of(total, start, workers) + 1; w <= last; w++)
-            if (stretch(total, w, workers) < stretch(total, w + 1, workers)) {
-                const long long at = (long long)w * rows + r;
-                add(more + at * HD, p.ml[more_ml + at]);
-            }
-    };
+    // The row's two segments: their first pieces by row, the others by worker (`more`: of which array, rows of a worker, row in them).
+    struct Segment {
+        int total, workers, from, to;            // pieces: the first, then workers from + 1 .. to
+        const float *first, *more;
+        long long first_ml, more_ml;
+        int rows, r;
+    } seg[2];
     {
         const int ts = t / p.tile_tokens, tile = ts * p.head_sets + hs, r = (t - ts * p.tile_tokens) * p.tile_heads + in;
-        if (tile < 2 * l.pairs)
-            pieces(l.pair_total, ((long long)hk * l.pairs + tile / 2) * l.nbp, l.nbp, ctas, p.first_prefix, 0, p.more_pair, 2 * all, 2 * kRows, (tile & 1) * kRows + r);
-        else
-            pieces(l.total, (long long)hk * l.nbp, l.nbp, 2 * ctas, p.first_prefix, 0, p.more, 2 * all + (long long)ctas * 2 * kRows, kRows, r);
+        const bool pair = tile < 2 * l.pairs;
+        Segment& x = seg[0];
+        x.total = pair ? l.pair_total : l.total;
+        x.workers = pair ? ctas : 2 * ctas;
+        const int start = pair ? (hk * l.pairs + tile / 2) * l.nbp : hk * l.nbp;
+        x.from = x.to = -1;
+        if (l.nbp > 0) {
+            x.from = worker_of(x.total, start, x.workers);
+            x.to = worker_of(x.total, start + l.nbp - 1, x.workers);
+        }
+        x.first = p.first_prefix;
+        x.first_ml = 0;
+        x.more = pair ? p.more_pair : p.more;
+        x.more_ml = 2 * all + (pair ? 0 : (long long)ctas * 2 * kRows);
+        x.rows = pair ? 2 * kRows : kRows;
+        x.r = pair ? (tile & 1) * kRows + r : r;
     }
     {
         const int dt = t - q.start, ts = dt / p.tile_tokens, tile = ts * p.head_sets + hs, r = (dt - ts * p.tile_tokens) * p.tile_heads + in;
-        pieces(l.total, l.odd + p.plan[lo] + ((long long)tile * p.kv_heads + hk) * q.blocks, q.blocks, 2 * ctas, p.first_own, all, p.more,
-               2 * all + (long long)ctas * 2 * kRows, kRows, r);
+        Segment& x = seg[1];
+        x.total = l.total;
+        x.workers = 2 * ctas;
+        const int start = l.odd + p.plan[lo] + (tile * p.kv_heads + hk) * q.blocks;
+        x.from = x.to = -1;
+        if (q.blocks > 0) {
+            x.from = worker_of(x.total, start, x.workers);
+            x.to = worker_of(x.total, start + q.blocks - 1, x.workers);
+        }
+        x.first = p.first_own;
+        x.first_ml = all;
+        x.more = p.more;
+        x.more_ml = 2 * all + (long long)ctas * 2 * kRows;
+        x.rows = kRows;
+        x.r = r;
     }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    T* dst = static_cast<T*>(p.out) + t * p.out_token + head * p.out_head + lane * N;
+    const int n0 = seg[0].from < 0 ? 0 : seg[0].to - seg[0].from + 1, n = n0 + (seg[1].from < 0 ? 0 : seg[1].to - seg[1].from + 1);
+    float m = -INFINITY, sum = 0.f, o[N] = {};
+#pragma unroll 1
+    for (int base = 0; base < n; base += 32) {
+        // a piece a lane (a worker whose stretch is empty has left none)
+        const int k = base + lane;
+        const float* src = nullptr;
+        float2 x = make_float2(-INFINITY, 0.f);
+        if (k < n) {
+            const Segment& s = k < n0 ? seg[0] : seg[1];
+            const int j = k < n0 ? k : k - n0, w = s.from + j;
+            if (j == 0) {
+                src = s.first + row * HD;
+                x = p.ml[s.first_ml + row];
+            } else if (stretch(s.total, w, s.workers) < stretch(s.total, w + 1, s.workers)) {
+                const long long at = (long long)w * s.rows + s.r;
+                src = s.more + at * HD;
+                x = p.ml[s.more_ml + at];
+            }
+        }
+        float top = x.x;
 #pragma unroll
-    for (int e = 0; e < N; e++) dst[e] = from_f32<T>(sum == 0.f ? 0.f : o[e] * inv);
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        if (top == -INFINITY) continue;
+        const float high = fmaxf(m, top), before = exp2_approx(m - high), weight = x.x == -INFINITY ? 0.f : exp2_approx(x.x - high);
+        float l2 = weight * x.y;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) l2 += __shfl_xor_sync(0xffffffffu, l2, d);
+        sum = sum * before + l2;
+        m = high;
+#pragma unroll
+        for (int e = 0; e < N; e++) o[e] *= before;
+        unsigned left = __ballot_sync(0xffffffffu, weight > 0.f || weight != weight);      // (NaN: scores of NaN make the row NaN)
+        while (left) {
+            float w[BATCH];
+            Vec<float, N> v[BATCH];
+#pragma unroll
+            for (int b = 0; b < BATCH; b++) {                            // (loads of several pieces in flight)
+                const int j = left ? __ffs(left) - 1 : 0;
+                const float* from = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), j));
+                w[b] = __shfl_sync(0xffffffffu, weight, j);
+                if (left) load_vec<true>(v[b], from + lane * N, N);
+                else w[b] = 0.f;
+                if (w[b] == 0.f)
+#pragma unroll
+                    for (int e = 0; e < N; e++) v[b].v[e] = 0.f;
+                left &= left - 1;
+            }
+#pragma unroll
+            for (int b = 0; b < BATCH; b++)
+#pragma unroll
+                for (int e = 0; e < N; e++) o[e] += w[b] * v[b].v[e];
+        }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    Vec<T, N> y;
+#pragma unroll
+    for (int e = 0; e < N; e++) y.v[e] = from_f32<T>(o[e] * inv);
+    store_vec<true>(static_cast<T*>(p.out) + t * p.out_token + head * p.out_head + lane * N, y, N);
 }
 
 struct Room {
@@ -803,10 +932,11 @@ int b200_paged_attention(const b200_paged* c, const void* q, long long q_token, 
     const int hd = c->head_dim, box = std::min(c->page_size, kKeys);
     const bool bf = c->dtype == B200_DTYPE_BF16;
     const CUtensorMapDataType type = bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    for (int one = 0; one < 2; one++) {
-        const int rc = make_map_3d(one ? &p.q1map : &p.qmap, type, q, hd, c->heads, c->tokens, stride_bytes(q_head, c->heads, hd),
-                                   stride_bytes(q_token, c->tokens, hd), 64, p.tile_heads, one ? 1 : p.tile_tokens, CU_TENSOR_MAP_SWIZZLE_128B,
-                                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
+    p.half_tokens = std::max(kRows / 2 / p.tile_heads, 1);              // (a head set of more than 64 rows is never half a tile)
+    for (int k = 0; k < 3; k++) {
+        const int rc = make_map_3d(k == 0 ? &p.qmap : (k == 1 ? &p.qhmap : &p.q1map), type, q, hd, c->heads, c->tokens, stride_bytes(q_head, c->heads, hd),
+                                   stride_bytes(q_token, c->tokens, hd), 64, p.tile_heads, k == 0 ? p.tile_tokens : (k == 1 ? p.half_tokens : 1),
+                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
         if (rc != B200_OK) return rc;
     }
     for (int v = 0; v < 2; v++) {
