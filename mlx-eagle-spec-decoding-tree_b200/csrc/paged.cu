@@ -4,8 +4,8 @@
 //
 // The softmax is split over its keys: a piece of them gives its maximum m, l = sum exp(s - m) and O = sum exp(s - m) v, and pieces are joined by
 // weights exp(m - max m) / sum.  A segment is the prefix with a tile of 128 query rows (token, head of the group) of any requests, or a request's
-// own rows with a tile of its tokens; its work is counted in blocks of 128 keys.  All blocks of all segments stand in one line, and every worker takes
-// an equal stretch of it, whatever the lengths: at most one piece a worker begins inside a segment, so a segment's first piece has its place by
+// own rows with a tile of its tokens; its work is counted in blocks of 128 keys.  All blocks of all segments stand in one line, and every worker
+// takes an equal stretch of it, whatever the lengths: at most one piece a worker begins inside a segment, so a segment's first piece has its place by
 // (token, head) and the others theirs by worker.  A second kernel joins them.
 //
 // One CTA an SM, two workers (streams) a CTA: eight warps each, two threads a query row, its scores and output in tensor memory (128 +
@@ -77,18 +77,13 @@ __device__ __forceinline__ Line line_of(const PagedParams& p, int own) {
     l.total = l.odd + own;
     return l;
 }
-// Where the stretch of worker i of n begins (n below 2^15).
-__device__ __forceinline__ int stretch(int total, int i, int n) {
-    const int q = total / n;
-    return q * i + (total - q * n) * i / n;
-}
-// The last worker of n whose stretch begins at block w or before.
-__device__ __forceinline__ int worker_of(int total, int w, int n) {
-    int i = min((int)((float)(w + 1) * (float)n / (float)total), n - 1);
-    while (i > 0 && stretch(total, i, n) > w) i--;
-    while (i + 1 < n && stretch(total, i + 1, n) <= w) i++;
-    return i;
-}
+// A line of blocks dealt out to workers in equal stretches, none of them empty: n of them, the first r of q + 1 blocks, the others of q.
+struct Share {
+    int total, n, q, r;
+    __device__ __forceinline__ Share(int total, int workers) : total(total), n(min(workers, total)), q(n ? total / n : 0), r(total - q * n) {}
+    __device__ __forceinline__ int start(int w) const { return w < n ? q * w + min(w, r) : total; }
+    __device__ __forceinline__ int owner(int b) const { return b < r * (q + 1) ? b / (q + 1) : r + (b - r * (q + 1)) / q; }
+};
 
 struct Request {
     int start, count, length, old;               // first token, tokens, rows, rows ahead of the pass's (as the lengths say, whatever the table holds)
@@ -295,7 +290,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
     pdl_launch_dependents();
     pdl_wait();
 
-    // ---- own blocks ahead of each request: consecutive requests a thread, then a scan (a line beyond 2^30 blocks is cut there)
+    // ---- own blocks ahead of each request: consecutive requests a thread, then a scan (a line beyond 2^28 blocks is cut there)
     {
         const int per = (p.requests + kPgThreads - 1) / kPgThreads, b0 = min((int)threadIdx.x * per, p.requests), b1 = min(b0 + per, p.requests);
         long long mine = 0, before;
@@ -315,24 +310,25 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
         before = scan - mine;
         for (int w = 0; w < warp; w++) before += s_warp[w];
         for (int b = b0; b < b1; b++) {
-            s_cum[b] = (int)min(before, 1ll << 30);
+            s_cum[b] = (int)min(before, 1ll << 28);
             before += (long long)s_req[b].blocks * s_req[b].tiles * p.kv_heads;
         }
-        if (threadIdx.x == kPgThreads - 1) s_cum[p.requests] = (int)min(before, 1ll << 30);
+        if (threadIdx.x == kPgThreads - 1) s_cum[p.requests] = (int)min(before, 1ll << 28);
         __syncthreads();
     }
     const Line l = line_of(p, s_cum[p.requests]);
-    // This CTA's stretch of the pairs, and its streams' of the rest.  Every other CTA begins with the rest: pairs keep the tensor cores busy, the
-    // rest the memory.
-    const int turn = cta & 1;
     if (threadIdx.x < 3) {
+        // (the streams' workers: first one of every CTA, then the other)
         const bool pair = threadIdx.x == 0;
-        const int total = pair ? l.pair_total : l.total, i = pair ? cta : 2 * cta + threadIdx.x - 1, n = pair ? ctas : 2 * ctas;
-        s_from[threadIdx.x] = cursor_at(p, l, s_cum, s_req, pair, stretch(total, i, n), stretch(total, i + 1, n));
+        const Share share(pair ? l.pair_total : l.total, pair ? ctas : 2 * ctas);
+        const int w = cta + (threadIdx.x == 2 ? ctas : 0);
+        s_from[threadIdx.x] = cursor_at(p, l, s_cum, s_req, pair, share.start(w), share.start(w + 1));
     } else if (cta == 0 && warp > 0) {
         for (int b = threadIdx.x - 32; b <= p.requests; b += kPgThreads - 32) p.plan[b] = s_cum[b];
     }
     __syncthreads();
+    // Blocks of pairs, of either stream.  Every other CTA begins with the latter: pairs keep the tensor cores busy, the rest the memory.
+    const int turn = cta & 1;
     const int np = uniform(s_from[0].end - s_from[0].w), n0 = uniform(s_from[1].end - s_from[1].w), n1 = uniform(s_from[2].end - s_from[2].w);
 
     if (warp == kKeyLoader || warp == kValueLoader) {
@@ -403,15 +399,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
             const uint32_t bar = smem_u32(full + slot), dst = slots + slot * G::SLOT;
             if (elect_one()) mbar_expect_tx(bar, boxes * p.box_rows * HD * 2);
             __syncwarp();
-#pragma unroll 1
-            for (int j = 0; j < boxes; j++) {
-                const int at = uniform(__shfl_sync(0xffffffffu, page, j));
-                if (elect_one()) {
-#pragma unroll
-                    for (int h = 0; h < NB; h++) tma_box4(dst + h * (kKeys * 128) + j * p.box_rows * 128, map, h * 64, row, hk, at, bar);
-                }
-                __syncwarp();
-            }
+            // (a box a lane, a page's next 64 dims in the lanes behind: from one thread, one after the other, they took half as long again)
+            const int at = __shfl_sync(0xffffffffu, page, lane & 15), h = lane >> 4;
+            if ((lane & 15) < boxes && h < NB) tma_box4(dst + h * (kKeys * 128) + (lane & 15) * p.box_rows * 128, map, h * 64, row, hk, at, bar);
+            __syncwarp();
             ring++;
             if (first && !values) {                                      // (behind the keys: their slot is free earlier)
                 if (s != 1) ask(0, x.c, x.c.tile);
@@ -687,7 +678,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
                     at = (c.req < 0 ? 0 : all) + row;
                 } else {
                     // (pairs: 256 rows a CTA; single streams: 128 a stream, behind them)
-                    const long long slot = (long long)cta * 2 * kRows + s * kRows + r;
+                    const long long slot = pair ? (long long)cta * 2 * kRows + s * kRows + r : ((long long)s * ctas + cta) * kRows + r;
                     dst = (pair ? p.more_pair : p.more) + slot * HD;
                     at = 2 * all + (pair ? 0 : (long long)ctas * 2 * kRows) + slot;
                 }
@@ -748,7 +739,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     const long long row = (long long)t * p.heads + head, all = (long long)p.tokens * p.heads;
     // The row's two segments: their first pieces by row, the others by worker (`more`: of which array, rows of a worker, row in them).
     struct Segment {
-        int total, workers, from, to;            // pieces: the first, then workers from + 1 .. to
+        int from, to;                            // pieces: the first, then workers from + 1 .. to
         const float *first, *more;
         long long first_ml, more_ml;
         int rows, r;
@@ -757,13 +748,12 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
         const int ts = t / p.tile_tokens, tile = ts * p.head_sets + hs, r = (t - ts * p.tile_tokens) * p.tile_heads + in;
         const bool pair = tile < 2 * l.pairs;
         Segment& x = seg[0];
-        x.total = pair ? l.pair_total : l.total;
-        x.workers = pair ? ctas : 2 * ctas;
+        const Share share(pair ? l.pair_total : l.total, pair ? ctas : 2 * ctas);
         const int start = pair ? (hk * l.pairs + tile / 2) * l.nbp : hk * l.nbp;
         x.from = x.to = -1;
         if (l.nbp > 0) {
-            x.from = worker_of(x.total, start, x.workers);
-            x.to = worker_of(x.total, start + l.nbp - 1, x.workers);
+            x.from = share.owner(start);
+            x.to = share.owner(start + l.nbp - 1);
         }
         x.first = p.first_prefix;
         x.first_ml = 0;
@@ -775,13 +765,12 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     {
         const int dt = t - q.start, ts = dt / p.tile_tokens, tile = ts * p.head_sets + hs, r = (dt - ts * p.tile_tokens) * p.tile_heads + in;
         Segment& x = seg[1];
-        x.total = l.total;
-        x.workers = 2 * ctas;
+        const Share share(l.total, 2 * ctas);
         const int start = l.odd + p.plan[lo] + (tile * p.kv_heads + hk) * q.blocks;
         x.from = x.to = -1;
         if (q.blocks > 0) {
-            x.from = worker_of(x.total, start, x.workers);
-            x.to = worker_of(x.total, start + q.blocks - 1, x.workers);
+            x.from = share.owner(start);
+            x.to = share.owner(start + q.blocks - 1);
         }
         x.first = p.first_own;
         x.first_ml = all;
@@ -794,7 +783,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     float m = -INFINITY, sum = 0.f, o[N] = {};
 #pragma unroll 1
     for (int base = 0; base < n; base += 32) {
-        // a piece a lane (a worker whose stretch is empty has left none)
+        // a piece a lane
         const int k = base + lane;
         const float* src = nullptr;
         float2 x = make_float2(-INFINITY, 0.f);
@@ -804,7 +793,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
             if (j == 0) {
                 src = s.first + row * HD;
                 x = p.ml[s.first_ml + row];
-            } else if (stretch(s.total, w, s.workers) < stretch(s.total, w + 1, s.workers)) {
+            } else {
                 const long long at = (long long)w * s.rows + s.r;
                 src = s.more + at * HD;
                 x = p.ml[s.more_ml + at];
@@ -928,7 +917,7 @@ int b200_paged_attention(const b200_paged* c, const void* q, long long q_token, 
     }
     // The line of blocks is counted in 32 bits.
     const double tiles = ((double)c->tokens / p.tile_tokens + c->requests + 1) * p.head_sets * c->kv_heads;
-    if (tiles * ((double)c->table_width * c->page_size / kKeys + prefix_length / kKeys + 2) > (double)(1 << 30)) return B200_ELIMIT;
+    if (tiles * ((double)c->table_width * c->page_size / kKeys + prefix_length / kKeys + 2) > (double)(1 << 28)) return B200_ELIMIT;
     const int hd = c->head_dim, box = std::min(c->page_size, kKeys);
     const bool bf = c->dtype == B200_DTYPE_BF16;
     const CUtensorMapDataType type = bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
