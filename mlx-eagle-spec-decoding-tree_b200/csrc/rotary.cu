@@ -59,13 +59,50 @@ __device__ __forceinline__ int find_request(const int* starts, int requests, int
 // An item is VE dims of one head (interleaved: VE / 2 pairs), or the VE pairs of two times VE dims.  WHOLE: all loads are of 16 bytes; else element
 // by element, for any strides and sizes.  What bounds it: launch latency up to a few MB, then HBM.
 template <typename T, int VE, bool WHOLE, bool INTERLEAVED, bool APPEND>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotParams p) {
+__global__ void __launch_bounds__(kRotThreads, 3) rotary_kernel(const RotParams p) {
     pdl_wait();
     pdl_launch_dependents();
-    extern __shared__ float2 turned[];                                   // [token][half]: magnitude * (cos, sin)
+    extern __shared__ __align__(16) float2 turned[];                                   // [token][half]: magnitude * (cos, sin)
     __shared__ long long s_pos[kRotTokens], s_row[kRotTokens];           // position; cache offset, -1: nowhere, -2: no request's token
     const int t0 = blockIdx.x * p.per_cta, toks = min(p.per_cta, p.tokens - t0);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int rot = p.half * 2, pair_items = (INTERLEAVED ? rot + VE - 1 : p.half + VE - 1) / VE;
+    const int head_items = pair_items + (p.dim - rot + VE - 1) / VE, heads = APPEND ? p.heads + 2 * p.kv_heads : p.heads;
+    // A thread keeps its place in the head and goes through heads and tokens, `step` heads a sweep: no division but one at the start.
+    const int cols = min(head_items, kRotThreads), sweep = kRotThreads / cols, mine = threadIdx.x / cols;
+    const int step = sweep * gridDim.y, h0 = blockIdx.y * sweep + mine;
+    int it = threadIdx.x - mine * cols;
+    struct At {
+        int t, h;
+    };
+    auto next = [&](At& x) {
+        x.h += step;
+        if (x.h >= heads) {
+            x.h = h0;
+            x.t++;
+        }
+    };
+    Vec<T, VE> a[kRotItems], b[kRotItems];
+    auto load = [&](At x) {
+        const bool pairs = it < pair_items;
+        const int c = pairs ? it * VE : rot + (it - pair_items) * VE, n = min((pairs ? (INTERLEAVED ? rot : p.half) : p.dim) - c, VE);
+#pragma unroll
+        for (int j = 0; j < kRotItems; j++, next(x)) {
+            if (x.t >= toks) break;
+            const Heads* from = &p.in;
+            int h = x.h;
+            if (APPEND && h >= p.heads) {
+                from = h < p.heads + p.kv_heads ? &p.k : &p.v;
+                h -= h < p.heads + p.kv_heads ? p.heads : p.heads + p.kv_heads;
+            }
+            const T* src = reinterpret_cast<const T*>(from->base) + (t0 + x.t) * from->token + h * from->head + c;
+            load_vec<WHOLE>(a[j], src, n);
+            if (!INTERLEAVED && pairs) load_vec<WHOLE>(b[j], src + p.half, n);
+        }
+    };
+    // Loads first: places and angles take as long as they do.
+    At at{h0 < heads && mine < sweep ? 0 : toks, h0};
+    load(at);
     if (warp < toks) {
         const int t = t0 + warp;
         long long row = 0, at = 0;
@@ -76,8 +113,8 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotParams p) 
                 row = (long long)p.lengths[r] - p.row_starts[r + 1] + t;
                 at = -1;
                 if (row >= 0 && row < (long long)p.table_width * p.page_size) {
-                    const int page = p.table[r * p.table_stride + row / p.page_size];
-                    if (page >= 0 && page < p.pages) at = page * p.page_stride + row % p.page_size * p.page_row;
+                    const int index = (int)row / p.page_size, page = p.table[r * p.table_stride + index];
+                    if (page >= 0 && page < p.pages) at = page * p.page_stride + ((int)row - index * p.page_size) * p.page_row;
                 }
             }
         }
@@ -89,7 +126,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotParams p) 
     }
     __syncthreads();
     for (int i = threadIdx.x; i < toks * p.half; i += kRotThreads) {
-        const int t = i / p.half;
+        const int t = p.per_cta == 1 ? 0 : i / p.half;
         double f = p.inv_freqs[i - t * p.half] * p.turns;
         f -= floor(f);
         const unsigned long long phase = __double2ull_rz(f * 0x1p64) * (unsigned long long)s_pos[t];
@@ -108,69 +145,59 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotParams p) 
         turned[i] = make_float2(c * p.magnitude, (p.inverse ? -s : s) * p.magnitude);
     }
     __syncthreads();
-
-    const int rot = p.half * 2, pair_items = ((INTERLEAVED ? rot : p.half) + VE - 1) / VE;
-    const int head_items = pair_items + (p.dim - rot + VE - 1) / VE;
-    const int heads = APPEND ? p.heads + 2 * p.kv_heads : p.heads, total = toks * heads * head_items;
-    const int stride = gridDim.y * kRotThreads;
-    for (int first = blockIdx.y * kRotThreads + threadIdx.x; first < total; first += stride * kRotItems) {
-        Vec<T, VE> a[kRotItems], b[kRotItems];
-        T* dst[kRotItems];
-        const float2* cs[kRotItems];                                     // NULL: passes through
-        int n[kRotItems];                                                // elements; negative: of either side
+    while (it < head_items) {                                            // (once, but for heads of more loads than there are threads)
+        const bool pairs = it < pair_items;
+        const int c = pairs ? it * VE : rot + (it - pair_items) * VE, n = min((pairs ? (INTERLEAVED ? rot : p.half) : p.dim) - c, VE);
+        while (at.t < toks) {
+            At x = at;
 #pragma unroll
-        for (int j = 0; j < kRotItems; j++) {
-            const int i = first + j * stride;
-            dst[j] = nullptr;
-            cs[j] = nullptr;
-            n[j] = 0;
-            if (i >= total) continue;
-            const int hd = i / head_items, it = i - hd * head_items, t = hd / heads;
-            int h = hd - t * heads;
-            const Heads* from = &p.in;
-            char* base = p.out.base;
-            long long to;
-            bool turn = it < pair_items;
-            if (!APPEND || h < p.heads) {
-                if (APPEND && s_row[t] == -2) continue;
-                to = (t0 + t) * p.out.token + h * p.out.head;
-            } else {
-                if (s_row[t] < 0) continue;
-                const bool is_k = h < p.heads + p.kv_heads;
-                h -= is_k ? p.heads : p.heads + p.kv_heads;
-                from = is_k ? &p.k : &p.v;
-                base = is_k ? p.k_pages : p.v_pages;
-                to = s_row[t] + h * p.page_head;
-                turn = turn && is_k;
-            }
-            const bool paired = !INTERLEAVED && it < pair_items;
-            const int c = it < pair_items ? it * VE : rot + (it - pair_items) * VE, left = (it >= pair_items ? p.dim : (INTERLEAVED ? rot : p.half)) - c;
-            const T* src = reinterpret_cast<const T*>(from->base) + (t0 + t) * from->token + h * from->head + c;
-            n[j] = paired ? -min(left, VE) : min(left, VE);
-            load_vec<WHOLE>(a[j], src, min(left, VE));
-            if (paired) load_vec<WHOLE>(b[j], src + p.half, min(left, VE));
-            dst[j] = reinterpret_cast<T*>(base) + to + c;
-            if (turn) cs[j] = turned + t * p.half + (INTERLEAVED ? c / 2 : c);
-        }
-#pragma unroll
-        for (int j = 0; j < kRotItems; j++) {
-            if (dst[j] == nullptr) continue;
-            const int count = abs(n[j]);
-            if (cs[j] != nullptr) {
-#pragma unroll
-                for (int e = 0; e < VE; e += INTERLEAVED ? 2 : 1) {
-                    if (!WHOLE && e >= count) break;
-                    const float2 w = cs[j][INTERLEAVED ? e / 2 : e];
-                    T& lo = a[j].v[e];
-                    T& hi = INTERLEAVED ? a[j].v[(e + 1) % VE] : b[j].v[e];
-                    const float x = to_f32(lo), y = to_f32(hi);
-                    lo = from_f32<T>(x * w.x - y * w.y);
-                    hi = from_f32<T>(x * w.y + y * w.x);
+            for (int j = 0; j < kRotItems; j++, next(x)) {
+                if (x.t >= toks) break;
+                char* base = p.out.base;
+                long long to = (t0 + x.t) * p.out.token + x.h * p.out.head;
+                bool turn = pairs;
+                if (APPEND) {
+                    const long long row = s_row[x.t];
+                    if (x.h < p.heads ? row == -2 : row < 0) continue;
+                    if (x.h >= p.heads) {
+                        const bool is_k = x.h < p.heads + p.kv_heads;
+                        base = is_k ? p.k_pages : p.v_pages;
+                        to = row + (x.h - (is_k ? p.heads : p.heads + p.kv_heads)) * p.page_head;
+                        turn = turn && is_k;
+                    }
                 }
+                if (turn) {
+                    constexpr int PAIRS = INTERLEAVED ? VE / 2 : VE;
+                    const float2* cs = turned + x.t * p.half + (INTERLEAVED ? c / 2 : c);
+                    Vec<float2, PAIRS> w;
+                    if constexpr (WHOLE) {
+#pragma unroll
+                        for (int e = 0; e < PAIRS; e += 2) *reinterpret_cast<float4*>(w.v + e) = *reinterpret_cast<const float4*>(cs + e);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < PAIRS; e++)
+                            if (e < n) w.v[e] = cs[e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < PAIRS; e++) {
+                        T& lo = a[j].v[INTERLEAVED ? 2 * e : e];
+                        T& hi = INTERLEAVED ? a[j].v[(2 * e + 1) % VE] : b[j].v[e];
+                        const float u = to_f32(lo), v = to_f32(hi);
+                        lo = from_f32<T>(u * w.v[e].x - v * w.v[e].y);
+                        hi = from_f32<T>(u * w.v[e].y + v * w.v[e].x);
+                    }
+                }
+                T* dst = reinterpret_cast<T*>(base) + to + c;
+                store_vec<WHOLE>(dst, a[j], n);
+                if (!INTERLEAVED && pairs) store_vec<WHOLE>(dst + p.half, b[j], n);
             }
-            store_vec<WHOLE>(dst[j], a[j], count);
-            if (n[j] < 0) store_vec<WHOLE>(dst[j] + p.half, b[j], count);
+            at = x;
+            load(at);
         }
+        it += cols;
+        if (it >= head_items) break;
+        at = {h0 < heads && mine < sweep ? 0 : toks, h0};
+        load(at);
     }
 }
 
@@ -186,13 +213,13 @@ int launch_rotary(RotParams& p, bool interleaved, cudaStream_t stream) {
         vec = vec && whole(p, p.k, VE) && whole(p, p.v, VE) && aligned16(p.k_pages) && aligned16(p.v_pages) && p.page_stride % VE == 0 &&
               p.page_head % VE == 0 && p.page_row % VE == 0;
     const int ve = vec ? VE : 2, heads = APPEND ? p.heads + 2 * p.kv_heads : p.heads;
-    const int items = heads * (((interleaved ? rot : p.half) + ve - 1) / ve + (p.dim - rot + ve - 1) / ve);
-    // Tokens of a CTA: so many that every thread has its loads in flight, as long as there are CTAs for all SMs; a token of many heads
-    // goes to several, whose number of waves counts the angles' share.
+    const int items = ((interleaved ? rot : p.half) + ve - 1) / ve + (p.dim - rot + ve - 1) / ve, sweep = std::max(kRotThreads / items, 1);
+    // Tokens of a CTA: so many that every thread has its loads in flight, as long as there are CTAs for all SMs; few tokens of many heads
+    // go to several CTAs each, a sweep of heads to each.
     p.per_cta = 1;
-    while (p.per_cta < kRotTokens && p.per_cta * items < kRotThreads * kRotItems && p.tokens / (2 * p.per_cta) >= 2 * 148) p.per_cta *= 2;
-    const int split = p.tokens >= 2 * 148 ? kRotItems : 1;               // (few tokens: a load a thread)
-    const int gy = std::min((p.per_cta * items + kRotThreads * split - 1) / (kRotThreads * split), 256);
+    while (p.per_cta < kRotTokens && p.per_cta * heads < sweep * kRotItems && p.tokens / (2 * p.per_cta) >= 4 * 148) p.per_cta *= 2;
+    const int sweeps = (heads + sweep - 1) / sweep;
+    const int gy = p.tokens >= 4 * 148 ? std::max(sweeps * p.per_cta / kRotItems, 1) : std::min(sweeps, 65535);
     const dim3 grid((p.tokens + p.per_cta - 1) / p.per_cta, gy);
     const size_t smem = sizeof(float2) * p.half * p.per_cta;
     auto go = [&](auto kern) { launch_kernel(kern, grid, dim3(kRotThreads), smem, stream, p); };

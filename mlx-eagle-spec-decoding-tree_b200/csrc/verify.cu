@@ -38,10 +38,44 @@ __device__ __forceinline__ double weight(T p, T q, bool less) {
     const double w = less ? (double)to_f32(p) - (double)to_f32(q) : (double)to_f32(p);
     return w > 0.0 ? w : 0.0;                    // (NaN weighs nothing)
 }
+// Sum of the weights of elements lo .. hi of a row by a warp, per lane; lo is a multiple of VE.
+template <typename T, int VE, bool LESS>
+__device__ __forceinline__ double lane_sum(const T* a, const T* b, int lo, int hi, int lane) {
+    constexpr int N = LESS ? 4 : 8;                                      // loads in flight, of either row
+    double sum[2] = {0.0, 0.0};
+    auto add = [&](const Vec<T, VE>& x, const Vec<T, VE>& y) {
+#pragma unroll
+        for (int e = 0; e < VE; e++) sum[e & 1] += weight(x.v[e], LESS ? y.v[e] : x.v[e], LESS);
+    };
+    int k = lo + lane * VE;
+#pragma unroll 1
+    for (; k + ((N - 1) * 32 + 1) * VE <= hi; k += N * 32 * VE) {
+        Vec<T, VE> x[N], y[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            load_vec<true>(x[j], a + k + j * 32 * VE, VE);
+            if (LESS) load_vec<true>(y[j], b + k + j * 32 * VE, VE);
+        }
+#pragma unroll
+        for (int j = 0; j < N; j++) add(x[j], y[j]);
+    }
+#pragma unroll 2
+    for (; k + VE <= hi; k += 32 * VE) {
+        Vec<T, VE> x, y;
+        load_vec<true>(x, a + k, VE);
+        if (LESS) load_vec<true>(y, b + k, VE);
+        add(x, y);
+    }
+    if (VE > 1) {                                                        // the last elements of the row
+        k = max(hi / VE * VE, lo) + lane;
+        if (k < hi) sum[0] += weight(a[k], LESS ? b[k] : a[k], LESS);
+    }
+    return sum[0] + sum[1];
+}
 
 // VE: elements of a load, of 16 bytes where every row starts at such, else one.
 template <typename T, int VE>
-__global__ void __launch_bounds__(kVerThreads) verify_kernel(const VerParams p) {
+__global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const VerParams p) {
     pdl_wait();
     pdl_launch_dependents();
     __shared__ double s_sums[kVerMaxCluster * kVerWarps];                // of all pieces of the row, in its order
@@ -77,7 +111,8 @@ __global__ void __launch_bounds__(kVerThreads) verify_kernel(const VerParams p) 
     __syncthreads();
     const int n = s_stand, pieces = cs * kVerWarps;
     bool less = n < len && p.draft != nullptr;
-    int skip = n < len && p.draft == nullptr ? tokens[n] : -1;
+    const int refused = n < len ? tokens[n] : -1;
+    int skip = p.draft == nullptr ? refused : -1;                        // weighs nothing
     const T* a = target + n * p.target_row;
     const T* b = less ? draft + n * p.draft_row : a;
     const int per = ((p.vocab + pieces - 1) / pieces + VE - 1) / VE * VE;                     // elements of a piece
@@ -86,32 +121,15 @@ __global__ void __launch_bounds__(kVerThreads) verify_kernel(const VerParams p) 
     double before = 0.0, border = 0.0;
     for (int round = 0; round < 2; round++) {
         const int mine = rank * kVerWarps + warp, lo = min(mine * per, p.vocab), hi = min(lo + per, p.vocab);
-        double sum = 0.0;
-        int at = lo + lane * VE;
-#pragma unroll 1
-        for (; at + VE <= hi; at += 32 * VE * 4) {
-            Vec<T, VE> x[4], y[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int k = at + j * 32 * VE;
-                if (k + VE <= hi) {
-                    load_vec<true>(x[j], a + k, VE);
-                    load_vec<true>(y[j], b + k, VE);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int k = at + j * 32 * VE;
-                if (k + VE <= hi) {
-#pragma unroll
-                    for (int e = 0; e < VE; e++)
-                        if (k + e != skip) sum += weight(x[j].v[e], y[j].v[e], less);
-                }
-            }
-        }
-        if (VE > 1) {                                                    // the last elements of the row
-            const int k = hi / VE * VE + lane;
-            if (hi == p.vocab && lo < hi && k < hi && k >= lo && k != skip) sum += weight(a[k], b[k], less);
+        double sum;
+        if (less) {
+            sum = lane_sum<T, VE, true>(a, b, lo, hi, lane);
+        } else if (skip >= lo && skip < hi) {                            // what lies around the load that holds the token, then that
+            const int from = skip / VE * VE, to = min(from + VE, hi);
+            sum = lane_sum<T, VE, false>(a, a, lo, from, lane) + lane_sum<T, VE, false>(a, a, to, hi, lane);
+            if (from + lane < to && from + lane != skip) sum += weight(a[from + lane], a[from + lane], false);
+        } else {
+            sum = lane_sum<T, VE, false>(a, a, lo, hi, lane);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -248,7 +266,9 @@ extern "C" int b200_verify_tokens(const int* draft_tokens, long long tokens_stri
     const int ve = (int)(16 / size);
     bool vec = b200::aligned16(target) && target_request % ve == 0 && target_row % ve == 0;
     if (draft) vec = vec && b200::aligned16(draft) && draft_request % ve == 0 && draft_row % ve == 0;
-    const int cluster = b200::kVerMaxCluster;
+    // As many CTAs a request as still run at once, two to an SM (64 requests of 152064 entries: XX us in clusters of 4, YY in clusters of 8).
+    int cluster = b200::kVerMaxCluster;
+    while (cluster > 1 && requests * cluster > 2 * 148) cluster /= 2;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == B200_DTYPE_F32) {
         if (vec) b200::launch_verify<float, 4>(p, requests, cluster, st);
