@@ -8,6 +8,7 @@
 // fraction of a turn of the product, whatever the position (53 bits of the product of doubles: 2^-37 turns at 131072 and a frequency of
 // one, where a product in single precision is off by 2^-9 radians).  Products and sums of a pair are fp32, rounded once to the result's type.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 #include "typed.cuh"
@@ -16,8 +17,8 @@ namespace b200 {
 namespace {
 
 constexpr int kRotThreads = 256;
-constexpr int kRotTokens = 4;                    // of a CTA, at most
-constexpr int kRotItems = 4;                     // loads of a thread in flight
+constexpr int kRotTokens = 2;                    // of a CTA, at most
+constexpr int kRotSweeps = 2;                    // of its threads over the heads, whose loads are in flight together
 
 // One block of heads that share addresses: head h of token t at base + t * token + h * head (elements).
 struct Heads {
@@ -59,7 +60,7 @@ __device__ __forceinline__ int find_request(const int* starts, int requests, int
 // An item is VE dims of one head (interleaved: VE / 2 pairs), or the VE pairs of two times VE dims.  WHOLE: all loads are of 16 bytes; else element
 // by element, for any strides and sizes.  What bounds it: launch latency up to a few MB, then HBM.
 template <typename T, int VE, bool WHOLE, bool INTERLEAVED, bool APPEND>
-__global__ void __launch_bounds__(kRotThreads, 3) rotary_kernel(const RotParams p) {
+__global__ void __launch_bounds__(kRotThreads, INTERLEAVED ? 4 : 3) rotary_kernel(const RotParams p) {
     pdl_wait();
     pdl_launch_dependents();
     extern __shared__ __align__(16) float2 turned[];                                   // [token][half]: magnitude * (cos, sin)
@@ -68,43 +69,46 @@ __global__ void __launch_bounds__(kRotThreads, 3) rotary_kernel(const RotParams 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rot = p.half * 2, pair_items = (INTERLEAVED ? rot + VE - 1 : p.half + VE - 1) / VE;
     const int head_items = pair_items + (p.dim - rot + VE - 1) / VE, heads = APPEND ? p.heads + 2 * p.kv_heads : p.heads;
-    // A thread keeps its place in the head and goes through heads and tokens, `step` heads a sweep: no division but one at the start.
+    // A thread keeps its place in the head and goes through the heads, `sweep` of them at a time: no division but one at the start.
     const int cols = min(head_items, kRotThreads), sweep = kRotThreads / cols, mine = threadIdx.x / cols;
-    const int step = sweep * gridDim.y, h0 = blockIdx.y * sweep + mine;
-    int it = threadIdx.x - mine * cols;
-    struct At {
-        int t, h;
+    const int h0 = blockIdx.y * (sweep * kRotSweeps) + mine, step = sweep * kRotSweeps * gridDim.y;
+    Vec<T, VE> a[kRotTokens][kRotSweeps], b[kRotTokens][kRotSweeps];
+    int it = mine < sweep ? threadIdx.x - mine * cols : head_items;
+    bool pairs;
+    int c, n;                                                            // the place: first dim, elements of a side
+    auto place = [&]() {
+        pairs = it < pair_items;
+        c = pairs ? it * VE : rot + (it - pair_items) * VE;
+        n = min((pairs ? (INTERLEAVED ? rot : p.half) : p.dim) - c, VE);
     };
-    auto next = [&](At& x) {
-        x.h += step;
-        if (x.h >= heads) {
-            x.h = h0;
-            x.t++;
-        }
-    };
-    Vec<T, VE> a[kRotItems], b[kRotItems];
-    auto load = [&](At x) {
-        const bool pairs = it < pair_items;
-        const int c = pairs ? it * VE : rot + (it - pair_items) * VE, n = min((pairs ? (INTERLEAVED ? rot : p.half) : p.dim) - c, VE);
+    auto load = [&](int first) {
 #pragma unroll
-        for (int j = 0; j < kRotItems; j++, next(x)) {
-            if (x.t >= toks) break;
-            const Heads* from = &p.in;
-            int h = x.h;
-            if (APPEND && h >= p.heads) {
-                from = h < p.heads + p.kv_heads ? &p.k : &p.v;
-                h -= h < p.heads + p.kv_heads ? p.heads : p.heads + p.kv_heads;
+        for (int s = 0; s < kRotSweeps; s++) {
+            int h = first + s * sweep;
+            if (h >= heads) break;
+            const T* src;
+            long long token = p.in.token;
+            if (!APPEND || h < p.heads) {
+                src = reinterpret_cast<const T*>(p.in.base) + h * p.in.head;
+            } else {
+                const bool is_k = h < p.heads + p.kv_heads;
+                src = reinterpret_cast<const T*>(is_k ? p.k.base : p.v.base) + (h - (is_k ? p.heads : p.heads + p.kv_heads)) * p.k.head;
+                token = p.k.token;
             }
-            const T* src = reinterpret_cast<const T*>(from->base) + (t0 + x.t) * from->token + h * from->head + c;
-            load_vec<WHOLE>(a[j], src, n);
-            if (!INTERLEAVED && pairs) load_vec<WHOLE>(b[j], src + p.half, n);
+            src += t0 * token + c;
+#pragma unroll
+            for (int k = 0; k < kRotTokens; k++)
+                if (k < toks) {
+                    load_vec<WHOLE>(a[k][s], src + k * token, n);
+                    if (!INTERLEAVED && pairs) load_vec<WHOLE>(b[k][s], src + k * token + p.half, n);
+                }
         }
     };
     // Loads first: places and angles take as long as they do.
-    At at{h0 < heads && mine < sweep ? 0 : toks, h0};
-    load(at);
-    if (warp < toks) {
-        const int t = t0 + warp;
+    place();
+    if (it < head_items) load(h0);
+    for (int k = warp; k < toks; k += kRotThreads / 32) {
+        const int t = t0 + k;
         long long row = 0, at = 0;
         if (APPEND) {
             at = -2;
@@ -119,8 +123,8 @@ __global__ void __launch_bounds__(kRotThreads, 3) rotary_kernel(const RotParams 
             }
         }
         if (lane == 0) {
-            s_row[warp] = at;
-            s_pos[warp] = p.positions == nullptr ? row + p.prefix
+            s_row[k] = at;
+            s_pos[k] = p.positions == nullptr ? row + p.prefix
                                                  : (p.pos64 ? static_cast<const long long*>(p.positions)[t] : (long long)static_cast<const int*>(p.positions)[t]);
         }
     }
@@ -145,59 +149,70 @@ __global__ void __launch_bounds__(kRotThreads, 3) rotary_kernel(const RotParams 
         turned[i] = make_float2(c * p.magnitude, (p.inverse ? -s : s) * p.magnitude);
     }
     __syncthreads();
-    while (it < head_items) {                                            // (once, but for heads of more loads than there are threads)
-        const bool pairs = it < pair_items;
-        const int c = pairs ? it * VE : rot + (it - pair_items) * VE, n = min((pairs ? (INTERLEAVED ? rot : p.half) : p.dim) - c, VE);
-        while (at.t < toks) {
-            At x = at;
+    auto store = [&](int first) {
+        constexpr int PAIRS = INTERLEAVED ? VE / 2 : VE;
 #pragma unroll
-            for (int j = 0; j < kRotItems; j++, next(x)) {
-                if (x.t >= toks) break;
-                char* base = p.out.base;
-                long long to = (t0 + x.t) * p.out.token + x.h * p.out.head;
+        for (int k = 0; k < kRotTokens; k++) {
+            if (k >= toks) break;
+            Vec<float2, PAIRS> w;                                        // of the place, for all heads
+            if (pairs) {
+                const float2* cs = turned + k * p.half + (INTERLEAVED ? c / 2 : c);
+                if constexpr (WHOLE) {
+#pragma unroll
+                    for (int e = 0; e < PAIRS; e += 2) *reinterpret_cast<float4*>(w.v + e) = *reinterpret_cast<const float4*>(cs + e);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < PAIRS; e++) w.v[e] = e < n ? cs[e] : make_float2(0.f, 0.f);
+                }
+            }
+            const long long row = APPEND ? s_row[k] : 0;
+#pragma unroll
+            for (int s = 0; s < kRotSweeps; s++) {
+                const int h = first + s * sweep;
+                if (h >= heads) break;
+                T* dst;
                 bool turn = pairs;
-                if (APPEND) {
-                    const long long row = s_row[x.t];
-                    if (x.h < p.heads ? row == -2 : row < 0) continue;
-                    if (x.h >= p.heads) {
-                        const bool is_k = x.h < p.heads + p.kv_heads;
-                        base = is_k ? p.k_pages : p.v_pages;
-                        to = row + (x.h - (is_k ? p.heads : p.heads + p.kv_heads)) * p.page_head;
-                        turn = turn && is_k;
-                    }
+                if (!APPEND || h < p.heads) {
+                    if (APPEND && row == -2) continue;
+                    dst = reinterpret_cast<T*>(p.out.base) + (t0 + k) * p.out.token + h * p.out.head + c;
+                } else {
+                    if (row < 0) continue;
+                    const bool is_k = h < p.heads + p.kv_heads;
+                    turn = turn && is_k;
+                    dst = reinterpret_cast<T*>(is_k ? p.k_pages : p.v_pages) + row + (h - (is_k ? p.heads : p.heads + p.kv_heads)) * p.page_head + c;
                 }
                 if (turn) {
-                    constexpr int PAIRS = INTERLEAVED ? VE / 2 : VE;
-                    const float2* cs = turned + x.t * p.half + (INTERLEAVED ? c / 2 : c);
-                    Vec<float2, PAIRS> w;
-                    if constexpr (WHOLE) {
+                    T *x = a[k][s].v, *y = b[k][s].v;
+                    if (INTERLEAVED) {
 #pragma unroll
-                        for (int e = 0; e < PAIRS; e += 2) *reinterpret_cast<float4*>(w.v + e) = *reinterpret_cast<const float4*>(cs + e);
+                        for (int e = 0; e < PAIRS; e++) {
+                            const float2 z = pair_of(x + 2 * e);
+                            set_pair(x + 2 * e, z.x * w.v[e].x - z.y * w.v[e].y, z.x * w.v[e].y + z.y * w.v[e].x);
+                        }
                     } else {
 #pragma unroll
-                        for (int e = 0; e < PAIRS; e++)
-                            if (e < n) w.v[e] = cs[e];
-                    }
-#pragma unroll
-                    for (int e = 0; e < PAIRS; e++) {
-                        T& lo = a[j].v[INTERLEAVED ? 2 * e : e];
-                        T& hi = INTERLEAVED ? a[j].v[(2 * e + 1) % VE] : b[j].v[e];
-                        const float u = to_f32(lo), v = to_f32(hi);
-                        lo = from_f32<T>(u * w.v[e].x - v * w.v[e].y);
-                        hi = from_f32<T>(u * w.v[e].y + v * w.v[e].x);
+                        for (int e = 0; e < PAIRS; e += 2) {             // (neighbours are rounded together)
+                            const float2 lo = pair_of(x + e), hi = pair_of(y + e), u = w.v[e], v = w.v[e + 1];
+                            set_pair(x + e, lo.x * u.x - hi.x * u.y, lo.y * v.x - hi.y * v.y);
+                            set_pair(y + e, lo.x * u.y + hi.x * u.x, lo.y * v.y + hi.y * v.x);
+                        }
                     }
                 }
-                T* dst = reinterpret_cast<T*>(base) + to + c;
-                store_vec<WHOLE>(dst, a[j], n);
-                if (!INTERLEAVED && pairs) store_vec<WHOLE>(dst + p.half, b[j], n);
+                store_vec<WHOLE>(dst, a[k][s], n);
+                if (!INTERLEAVED && pairs) store_vec<WHOLE>(dst + p.half, b[k][s], n);
             }
-            at = x;
-            load(at);
+        }
+    };
+    while (it < head_items) {                                            // (once, but for heads of more places than there are threads)
+        for (int h = h0; h < heads;) {
+            store(h);
+            h += step;
+            if (h < heads) load(h);
         }
         it += cols;
         if (it >= head_items) break;
-        at = {h0 < heads && mine < sweep ? 0 : toks, h0};
-        load(at);
+        place();
+        load(h0);
     }
 }
 
@@ -214,12 +229,9 @@ int launch_rotary(RotParams& p, bool interleaved, cudaStream_t stream) {
               p.page_head % VE == 0 && p.page_row % VE == 0;
     const int ve = vec ? VE : 2, heads = APPEND ? p.heads + 2 * p.kv_heads : p.heads;
     const int items = ((interleaved ? rot : p.half) + ve - 1) / ve + (p.dim - rot + ve - 1) / ve, sweep = std::max(kRotThreads / items, 1);
-    // Tokens of a CTA: so many that every thread has its loads in flight, as long as there are CTAs for all SMs; few tokens of many heads
-    // go to several CTAs each, a sweep of heads to each.
-    p.per_cta = 1;
-    while (p.per_cta < kRotTokens && p.per_cta * heads < sweep * kRotItems && p.tokens / (2 * p.per_cta) >= 4 * 148) p.per_cta *= 2;
-    const int sweeps = (heads + sweep - 1) / sweep;
-    const int gy = p.tokens >= 4 * 148 ? std::max(sweeps * p.per_cta / kRotItems, 1) : std::min(sweeps, 65535);
+    // Two tokens a CTA where there are CTAs enough; where there are few, the heads of one go to several.
+    p.per_cta = p.tokens >= 8 * 148 ? kRotTokens : 1;
+    const int gy = p.tokens >= 2 * 148 ? 1 : std::min((heads + sweep * kRotSweeps - 1) / (sweep * kRotSweeps), 65535);
     const dim3 grid((p.tokens + p.per_cta - 1) / p.per_cta, gy);
     const size_t smem = sizeof(float2) * p.half * p.per_cta;
     auto go = [&](auto kern) { launch_kernel(kern, grid, dim3(kRotThreads), smem, stream, p); };

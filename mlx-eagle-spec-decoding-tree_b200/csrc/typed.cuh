@@ -15,6 +15,17 @@ template <> __device__ __forceinline__ float from_f32<float>(float x) { return x
 template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// Two neighbours (at an even place, by whole words of memory), rounded together.
+__device__ __forceinline__ float2 pair_of(const float* p) { return make_float2(p[0], p[1]); }
+__device__ __forceinline__ float2 pair_of(const __half* p) { return __half22float2(*reinterpret_cast<const __half2*>(p)); }
+__device__ __forceinline__ float2 pair_of(const __nv_bfloat16* p) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ void set_pair(float* p, float x, float y) { p[0] = x; p[1] = y; }
+__device__ __forceinline__ void set_pair(__half* p, float x, float y) { *reinterpret_cast<__half2*>(p) = __floats2half2_rn(x, y); }
+__device__ __forceinline__ void set_pair(__nv_bfloat16* p, float x, float y) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(x, y); }
+
 // N elements: one access of N * sizeof(T) bytes (WHOLE), or the first `n` of them one by one.
 template <typename T, int N>
 struct alignas(N * sizeof(T)) Vec {
