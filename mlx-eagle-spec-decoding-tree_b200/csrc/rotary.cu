@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotTokens = 2;                    // of a CTA, at most
+static_assert(kRotTokens == 2, "which token an angle is for is a comparison");
 constexpr int kRotSweeps = 2;                    // of its threads over the heads, whose loads are in flight together
 
 // One block of heads that share addresses: head h of token t at base + t * token + h * head (elements).
@@ -57,6 +58,26 @@ __device__ __forceinline__ int find_request(const int* starts, int requests, int
     return lo;
 }
 
+// magnitude * (cos, sin) of frequency i at a position.
+__device__ __forceinline__ float2 turn_of(const RotParams& p, int i, long long pos) {
+    double f = p.inv_freqs[i] * p.turns;
+    f -= floor(f);
+    const unsigned long long phase = __double2ull_rz(f * 0x1p64) * (unsigned long long)pos;
+    const unsigned quarter = (unsigned)((phase + (1ull << 61)) >> 62);                       // the nearest quarter of a turn, what is left to either side
+    float s, c;
+    sincospif((float)(long long)(phase - ((unsigned long long)quarter << 62)) * 0x1p-63f, &s, &c);
+    if (quarter & 1) {
+        const float x = s;
+        s = c;
+        c = -x;
+    }
+    if (quarter & 2) {
+        s = -s;
+        c = -c;
+    }
+    return make_float2(c * p.magnitude, (p.inverse ? -s : s) * p.magnitude);
+}
+
 // An item is VE dims of one head (interleaved: VE / 2 pairs), or the VE pairs of two times VE dims.  WHOLE: all loads are of 16 bytes; else element
 // by element, for any strides and sizes.  What bounds it: launch latency up to a few MB, then HBM.
 template <typename T, int VE, bool WHOLE, bool INTERLEAVED, bool APPEND>
@@ -64,7 +85,7 @@ __global__ void __launch_bounds__(kRotThreads, INTERLEAVED ? 4 : 3) rotary_kerne
     pdl_wait();
     pdl_launch_dependents();
     extern __shared__ __align__(16) float2 turned[];                                   // [token][half]: magnitude * (cos, sin)
-    __shared__ long long s_pos[kRotTokens], s_row[kRotTokens];           // position; cache offset, -1: nowhere, -2: no request's token
+    __shared__ long long s_row[kRotTokens];                              // cache offset, -1: nowhere, -2: no request's token
     const int t0 = blockIdx.x * p.per_cta, toks = min(p.per_cta, p.tokens - t0);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rot = p.half * 2, pair_items = (INTERLEAVED ? rot + VE - 1 : p.half + VE - 1) / VE;
@@ -107,46 +128,30 @@ __global__ void __launch_bounds__(kRotThreads, INTERLEAVED ? 4 : 3) rotary_kerne
     // Loads first: places and angles take as long as they do.
     place();
     if (it < head_items) load(h0);
-    for (int k = warp; k < toks; k += kRotThreads / 32) {
-        const int t = t0 + k;
-        long long row = 0, at = 0;
-        if (APPEND) {
-            at = -2;
+    auto given = [&](int t) { return p.pos64 ? static_cast<const long long*>(p.positions)[t] : (long long)static_cast<const int*>(p.positions)[t]; };
+    if constexpr (!APPEND) {
+        for (int i = threadIdx.x; i < toks * p.half; i += kRotThreads) {
+            const int k = i >= p.half;                                   // (two tokens at most)
+            turned[i] = turn_of(p, i - k * p.half, given(t0 + k));
+        }
+    } else {
+        // Four warps a token (all, if there is one), each of which looks for the token's place itself, so that nothing waits in between.
+        const int per = kRotThreads / 32 / p.per_cta, k = warp / per, sub = warp - k * per, t = t0 + k;
+        if (k < toks) {
+            long long row = 0, at = -2;
             if (t >= p.row_starts[0] && t < p.row_starts[p.requests]) {
                 const int r = find_request(p.row_starts, p.requests, t, lane);
                 row = (long long)p.lengths[r] - p.row_starts[r + 1] + t;
                 at = -1;
-                if (row >= 0 && row < (long long)p.table_width * p.page_size) {
+                if (sub == 0 && row >= 0 && row < (long long)p.table_width * p.page_size) {
                     const int index = (int)row / p.page_size, page = p.table[r * p.table_stride + index];
                     if (page >= 0 && page < p.pages) at = page * p.page_stride + ((int)row - index * p.page_size) * p.page_row;
                 }
             }
+            if (sub == 0 && lane == 0) s_row[k] = at;
+            const long long pos = p.positions == nullptr ? row + p.prefix : given(t);
+            for (int i = sub * 32 + lane; i < p.half; i += per * 32) turned[k * p.half + i] = turn_of(p, i, pos);
         }
-        if (lane == 0) {
-            s_row[k] = at;
-            s_pos[k] = p.positions == nullptr ? row + p.prefix
-                                                 : (p.pos64 ? static_cast<const long long*>(p.positions)[t] : (long long)static_cast<const int*>(p.positions)[t]);
-        }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < toks * p.half; i += kRotThreads) {
-        const int t = p.per_cta == 1 ? 0 : i / p.half;
-        double f = p.inv_freqs[i - t * p.half] * p.turns;
-        f -= floor(f);
-        const unsigned long long phase = __double2ull_rz(f * 0x1p64) * (unsigned long long)s_pos[t];
-        const unsigned quarter = (unsigned)((phase + (1ull << 61)) >> 62);                   // the nearest quarter of a turn, what is left to either side
-        float s, c;
-        sincospif((float)(long long)(phase - ((unsigned long long)quarter << 62)) * 0x1p-63f, &s, &c);
-        if (quarter & 1) {
-            const float x = s;
-            s = c;
-            c = -x;
-        }
-        if (quarter & 2) {
-            s = -s;
-            c = -c;
-        }
-        turned[i] = make_float2(c * p.magnitude, (p.inverse ? -s : s) * p.magnitude);
     }
     __syncthreads();
     auto store = [&](int first) {
