@@ -31,9 +31,9 @@ namespace {
 constexpr int kKeys = 128;                       // of a block
 constexpr int kRows = 128;                       // query rows of a tile
 constexpr int kParts = 2;                        // threads of a query row
-constexpr int kPgThreads = 640;                  // 2 x 8 softmax warps, keys and queries, products, values (a warp idles)
+constexpr int kPgThreads = 576;                  // 2 x 8 softmax warps, copies, products: few enough for 112 registers a thread
 constexpr int kPgMaxRequests = 1024;
-constexpr int kKeyLoader = 16, kIssuer = 17, kValueLoader = 18;
+constexpr int kLoader = 16, kIssuer = 17;
 constexpr float kLag = 8.f;                      // a row's maximum may exceed its reference by 2^8
 
 template <int HD>
@@ -41,6 +41,22 @@ struct PGeo {
     static constexpr int QTILE = kRows * HD * 2, SLOT = kKeys * HD * 2, SLOTS = HD == 128 ? 2 : 4;      // of keys, and of values
     static constexpr int KV0 = 2 * QTILE, END = KV0 + 2 * SLOTS * SLOT;
     static constexpr int SMEM = END + 1024;
+};
+
+// A line of blocks dealt out to workers in equal stretches, none of them empty: n of them, the first r of q + 1 blocks, the others of q.
+struct Share {
+    int total, n, q, r;
+    __host__ __device__ Share() {}
+    __host__ __device__ __forceinline__ Share(int total, int workers)
+        : total(total), n(workers < total ? workers : total), q(n ? total / n : 0), r(total - q * n) {}
+    __device__ __forceinline__ int start(int w) const { return w < n ? q * w + min(w, r) : total; }
+    __device__ __forceinline__ int owner(int b) const { return b < r * (q + 1) ? b / (q + 1) : r + (b - r * (q + 1)) / q; }
+};
+// Blocks of the prefix, its query tiles (per kv head) and pairs of them; its blocks for tiles without a partner, which head the line of
+// single streams; the line of pairs and its workers.
+struct Line {
+    int nbp, tiles, pairs, odd;
+    Share pair;
 };
 
 struct PagedParams {
@@ -53,36 +69,13 @@ struct PagedParams {
     int* plan;                                   // sums of the own blocks, by request
     long long table_stride, out_token, out_head;
     int requests, tokens, heads, kv_heads, group, tile_heads, tile_tokens, half_tokens, head_sets;
-    int page_size, box_rows, table_width, prefix;
+    int page_size, page_shift, page_blocks;      // a page's rows; their logarithm, or the page's blocks if it is more than one
+    int box_rows, table_width, prefix;
+    Line line;
     float scale_log2;                            // positive
     bool negative;                               // ... of a negative scale
     int* err;
     int polls;
-};
-
-// The line of blocks.
-struct Line {
-    int nbp;                                     // blocks of the prefix
-    int tiles, pairs;                            // query tiles of the prefix, per kv head
-    int odd;                                     // blocks of prefix segments without a partner
-    int pair_total, total;                       // blocks for pairs; for single streams: odd ones, then own ones
-};
-__device__ __forceinline__ Line line_of(const PagedParams& p, int own) {
-    Line l;
-    l.nbp = (p.prefix + kKeys - 1) / kKeys;
-    l.tiles = (p.tokens + p.tile_tokens - 1) / p.tile_tokens * p.head_sets;
-    l.pairs = l.tiles / 2;
-    l.odd = l.tiles & 1 ? p.kv_heads * l.nbp : 0;
-    l.pair_total = p.kv_heads * l.pairs * l.nbp;
-    l.total = l.odd + own;
-    return l;
-}
-// A line of blocks dealt out to workers in equal stretches, none of them empty: n of them, the first r of q + 1 blocks, the others of q.
-struct Share {
-    int total, n, q, r;
-    __device__ __forceinline__ Share(int total, int workers) : total(total), n(min(workers, total)), q(n ? total / n : 0), r(total - q * n) {}
-    __device__ __forceinline__ int start(int w) const { return w < n ? q * w + min(w, r) : total; }
-    __device__ __forceinline__ int owner(int b) const { return b < r * (q + 1) ? b / (q + 1) : r + (b - r * (q + 1)) / q; }
 };
 
 struct Request {
@@ -97,7 +90,7 @@ __device__ __forceinline__ Request request_of(const PagedParams& p, int b) {
     r.length = (int)min((long long)max(len, 0), (long long)p.table_width * p.page_size);
     r.old = len - (s1 - s0);
     r.blocks = (r.length + kKeys - 1) / kKeys;
-    r.tiles = (r.count + p.tile_tokens - 1) / p.tile_tokens * p.head_sets;
+    r.tiles = (r.count <= p.tile_tokens ? min(r.count, 1) : (r.count + p.tile_tokens - 1) / p.tile_tokens) * p.head_sets;
     return r;
 }
 
@@ -117,7 +110,8 @@ __device__ __forceinline__ void enter(Cursor& c, const Request* reqs, int req) {
     c.tile = c.hk = c.kb = 0;
 }
 // The cursor of block w of the line of pairs (its tile is the first stream's) or of single streams; cum: own blocks ahead of each request.
-__device__ __forceinline__ Cursor cursor_at(const PagedParams& p, const Line& l, const int* cum, const Request* reqs, bool pair, int w, int end) {
+__device__ __forceinline__ Cursor cursor_at(const PagedParams& p, const int* cum, const Request* reqs, bool pair, int w, int end) {
+    const Line& l = p.line;
     Cursor c{};
     c.w = w;
     c.end = end;
@@ -147,7 +141,7 @@ __device__ __forceinline__ Cursor cursor_at(const PagedParams& p, const Line& l,
     return c;
 }
 // Past its piece.
-__device__ __forceinline__ void advance(Cursor& c, const PagedParams& p, const Line& l, const Request* reqs, bool pair) {
+__device__ __forceinline__ void advance(Cursor& c, const PagedParams& p, const Request* reqs, bool pair) {
     const int n = c.last() - c.kb;
     c.w += n;
     c.kb += n;
@@ -155,7 +149,7 @@ __device__ __forceinline__ void advance(Cursor& c, const PagedParams& p, const L
     c.kb = 0;
     if (pair) {
         c.tile += 2;
-        if (c.tile < 2 * l.pairs) return;
+        if (c.tile < 2 * p.line.pairs) return;
         c.tile = 0;
         c.hk++;
         return;
@@ -289,6 +283,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
     const uint32_t tmem = s_tmem;
     pdl_launch_dependents();
     pdl_wait();
+    // (what earlier kernels wrote by ordinary stores, rows and queries: 2000 cycles, of which all but a few pass behind the scan below)
+    if (warp == kLoader) asm volatile("fence.proxy.async;\n" ::: "memory");
 
     // ---- own blocks ahead of each request: consecutive requests a thread, then a scan (a line beyond 2^28 blocks is cut there)
     {
@@ -316,29 +312,23 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
         if (threadIdx.x == kPgThreads - 1) s_cum[p.requests] = (int)min(before, 1ll << 28);
         __syncthreads();
     }
-    const Line l = line_of(p, s_cum[p.requests]);
-    if (threadIdx.x < 3) {
+    if (warp < 3 && lane == 0) {
         // (the streams' workers: first one of every CTA, then the other)
-        const bool pair = threadIdx.x == 0;
-        const Share share(pair ? l.pair_total : l.total, pair ? ctas : 2 * ctas);
-        const int w = cta + (threadIdx.x == 2 ? ctas : 0);
-        s_from[threadIdx.x] = cursor_at(p, l, s_cum, s_req, pair, share.start(w), share.start(w + 1));
-    } else if (cta == 0 && warp > 0) {
-        for (int b = threadIdx.x - 32; b <= p.requests; b += kPgThreads - 32) p.plan[b] = s_cum[b];
+        const bool pair = warp == 0;
+        const Share share = pair ? p.line.pair : Share(p.line.odd + s_cum[p.requests], 2 * ctas);
+        const int w = cta + (warp == 2 ? ctas : 0);
+        s_from[warp] = cursor_at(p, s_cum, s_req, pair, share.start(w), share.start(w + 1));
+    } else if (cta == 0 && warp >= 3) {
+        for (int b = threadIdx.x - 96; b <= p.requests; b += kPgThreads - 96) p.plan[b] = s_cum[b];
     }
     __syncthreads();
     // Blocks of pairs, of either stream.  Every other CTA begins with the latter: pairs keep the tensor cores busy, the rest the memory.
     const int turn = cta & 1;
     const int np = uniform(s_from[0].end - s_from[0].w), n0 = uniform(s_from[1].end - s_from[1].w), n1 = uniform(s_from[2].end - s_from[2].w);
 
-    if (warp == kKeyLoader || warp == kValueLoader) {
-        // ------------------------------------------------------------------ keys and queries, or values, in the order of their use
-        asm volatile("fence.proxy.async;\n" ::: "memory");               // (appended by ordinary stores of an earlier kernel)
-        const bool values = warp == kValueLoader;
-        const CUtensorMap* map = values ? &p.vmap : &p.kmap;
-        uint64_t *const full = values ? vfull : kfull, *const free = values ? vfree : kfree;
-        const uint32_t slots = sbase + G::KV0 + (values ? ST * G::SLOT : 0);
-        int ring = 0;
+    if (warp == kLoader) {
+        // ------------------------------------------------------------------ keys, queries and values, in the order of their use
+        int kring = 0, vring = 0;
         int asked[4] = {0, 0, 0, 0}, half = 3;                           // uses of the streams' halves of queries; the halves last taken, a bit a stream
         // A tile of queries, or, of 64 rows at most, one of its halves in turn, so that the next piece's come while this one's are in use.
         auto ask = [&](int s, const Cursor& c, int tile) {
@@ -373,13 +363,16 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
         struct At {
             Cursor c;
             int kb, kb1;                                                 // of the piece
-            int ahead;                                                   // a page of the next block a lane
+            int page, ahead;                                             // pages a lane: of the block whose keys came last, of the next
+            int boxes, row, hk;                                          // ... its boxes, first row in its page, head
         };
         auto page_at = [&](const At& x, int kb) {
-            const int key = kb * kKeys + lane * p.box_rows;
+            const int key = kb * kKeys + (lane & 15) * p.box_rows;
             int page = 0;
-            if (lane * p.box_rows < kKeys && key < x.c.r.length && kb < x.kb1)
-                page = x.c.req < 0 ? p.prefix_pages[key / p.page_size] : p.table[x.c.req * p.table_stride + key / p.page_size];
+            if ((lane & 15) * p.box_rows < kKeys && key < x.c.r.length && kb < x.kb1) {
+                const int index = p.page_blocks > 1 ? kb / p.page_blocks : key >> p.page_shift;
+                page = x.c.req < 0 ? p.prefix_pages[index] : p.table[x.c.req * p.table_stride + index];
+            }
             return page;
         };
         auto start = [&](At& x, int which) {
@@ -388,28 +381,40 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
             x.kb1 = x.c.last();
             x.ahead = page_at(x, x.kb);
         };
-        // The cursor's next block; s: the stream that uses it, 2: both.
-        auto next = [&](At& x, int s) {
-            const bool first = x.kb == x.c.kb;
-            const int page = x.ahead, key0 = x.kb * kKeys, row = uniform(p.page_size > kKeys ? key0 % p.page_size : 0), hk = uniform(x.c.hk);
-            const int boxes = uniform((min(kKeys, x.c.r.length - key0) + p.box_rows - 1) / p.box_rows), slot = ring % ST;
-            x.ahead = page_at(x, x.kb + 1);
-            if (ring >= ST) mbar_wait_reported(smem_u32(free + slot), (ring / ST - 1) & 1, p.polls, p.err, 31);
-            __syncwarp();
-            const uint32_t bar = smem_u32(full + slot), dst = slots + slot * G::SLOT;
-            if (elect_one()) mbar_expect_tx(bar, boxes * p.box_rows * HD * 2);
+        auto copy = [&](const At& x, const CUtensorMap* map, uint32_t bar, uint32_t dst) {
+            if (elect_one()) mbar_expect_tx(bar, x.boxes * p.box_rows * HD * 2);
             __syncwarp();
             // (a box a lane, a page's next 64 dims in the lanes behind: from one thread, one after the other, they took half as long again)
-            const int at = __shfl_sync(0xffffffffu, page, lane & 15), h = lane >> 4;
-            if ((lane & 15) < boxes && h < NB) tma_box4(dst + h * (kKeys * 128) + (lane & 15) * p.box_rows * 128, map, h * 64, row, hk, at, bar);
+            if ((lane & 15) < x.boxes && lane >> 4 < NB)
+                tma_box4(dst + (lane >> 4) * (kKeys * 128) + (lane & 15) * p.box_rows * 128, map, (lane >> 4) * 64, x.row, x.hk, x.page, bar);
             __syncwarp();
-            ring++;
-            if (first && !values) {                                      // (behind the keys: their slot is free earlier)
+        };
+        auto values = [&](At& x) {                                       // of the block whose keys came last
+            const int slot = vring % ST;
+            if (vring >= ST) mbar_wait_reported(smem_u32(vfree + slot), (vring / ST - 1) & 1, p.polls, p.err, 31);
+            __syncwarp();
+            copy(x, &p.vmap, smem_u32(vfull + slot), sbase + G::KV0 + (ST + slot) * G::SLOT);
+            vring++;
+        };
+        // Keys of the cursor's next block, and the queries of its piece; s: the stream that uses it, 2: both.
+        auto keys = [&](At& x, int s) {
+            const bool first = x.kb == x.c.kb;
+            const int key0 = x.kb * kKeys, slot = kring % ST;
+            x.page = x.ahead;
+            x.row = p.page_blocks > 1 ? x.kb % p.page_blocks * kKeys : 0;
+            x.hk = x.c.hk;
+            x.boxes = (min(kKeys, x.c.r.length - key0) + p.box_rows - 1) / p.box_rows;
+            x.ahead = page_at(x, x.kb + 1);
+            if (kring >= ST) mbar_wait_reported(smem_u32(kfree + slot), (kring / ST - 1) & 1, p.polls, p.err, 31);
+            __syncwarp();
+            copy(x, &p.kmap, smem_u32(kfull + slot), sbase + G::KV0 + slot * G::SLOT);
+            kring++;
+            if (first) {                                                 // (behind the keys: their slot is free earlier)
                 if (s != 1) ask(0, x.c, x.c.tile);
                 if (s != 0) ask(1, x.c, x.c.tile + (s == 2));
             }
             if (++x.kb == x.kb1) {
-                advance(x.c, p, l, s_req, s == 2);
+                advance(x.c, p, s_req, s == 2);
                 x.kb = x.c.kb;
                 x.kb1 = x.c.last();
                 x.ahead = page_at(x, x.kb);
@@ -421,14 +426,29 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
             if (phase == turn) {
                 if (np > 0) start(x, 0);
 #pragma unroll 1
-                for (int i = 0; i < np; i++) next(x, 2);
+                for (int i = 0; i < np; i++) {
+                    keys(x, 2);
+                    values(x);
+                }
             } else {
-                if (n0 > 0) start(x, 1);
-                if (n1 > 0) start(y, 2);
+                if (n0 > 0) {
+                    start(x, 1);
+                    keys(x, 0);
+                }
+                if (n1 > 0) {
+                    start(y, 2);
+                    keys(y, 1);
+                }
 #pragma unroll 1
                 for (int i = 0; i < max(n0, n1); i++) {
-                    if (i < n0) next(x, 0);
-                    if (i < n1) next(y, 1);
+                    if (i < n0) {
+                        values(x);
+                        if (i + 1 < n0) keys(x, 0);
+                    }
+                    if (i < n1) {
+                        values(y);
+                        if (i + 1 < n1) keys(y, 1);
+                    }
                 }
             }
         }
@@ -487,7 +507,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
             __syncwarp();
             x.blocks++;
             if (give) kring++;
-            if (last) advance(x.c, p, l, s_req, pair);
+            if (last) advance(x.c, p, s_req, pair);
         };
         // Output of the block whose scores stream s asked for last.
         auto output = [&](int s, const At& x, bool take, bool give) {
@@ -549,9 +569,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
                     if (at[s].left > 0) scores(s, at[s], pair, !pair || s == 0, !pair || s == 1);
                 }
         }
-    } else if (warp < kKeyLoader) {
+    } else {
         // ------------------------------------------------------------------ softmax: 64 keys of a block of a query row a thread
-        constexpr int KEYS = kKeys / kParts, HALF = KEYS / 2, DIMS = HD / kParts;
+        constexpr int KEYS = kKeys / kParts, DIMS = HD / kParts;
+        static_assert(KEYS == 64, "a row's thread has a word of keys");
         const int s = warp >> 3, part = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tS = tmem + s * kKeys + part * KEYS + lanes, tO = tmem + 2 * kKeys + s * HD + part * DIMS + lanes;
         const int dt = r / p.tile_heads;
@@ -578,40 +599,37 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                 if (busy) {
                     const int key0 = kb * kKeys + part * KEYS;
-                    // Half of the scores at a time; what the row does not see is minus infinity.
-                    float a[HALF];
-                    auto scores = [&](int h) {
-                        uint32_t raw[HALF];
-                        tmem_ld32(raw, tS + h * HALF);
+                    float a[KEYS];
+                    {
+                        uint32_t raw[KEYS];
+                        tmem_ld32(raw, tS);
+                        tmem_ld32(raw + 32, tS + 32);
                         asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
-                        for (int j = 0; j < HALF; j++) a[j] = __uint_as_float(raw[j]);
-                        if (p.negative) {
+                        for (int j = 0; j < KEYS; j++) a[j] = __uint_as_float(raw[j]);
+                    }
+                    if (p.negative) {
 #pragma unroll
-                            for (int j = 0; j < HALF; j++) a[j] = -a[j];
-                        }
-                        const int k0 = key0 + h * HALF;
-                        if (k0 + HALF > sure) {
-                            const int o = k0 - old, there = length - k0, n = limit - k0;      // the first key among the new rows; keys there are; keys seen
-                            uint32_t seen = n >= HALF ? ~0u : (n <= 0 ? 0u : (1u << n) - 1);
-                            if (masked && o > -HALF && o < 64) seen |= (uint32_t)(o >= 0 ? bits >> o : bits << -o) & (there >= HALF ? ~0u : (there <= 0 ? 0u : (1u << there) - 1));
+                        for (int j = 0; j < KEYS; j++) a[j] = -a[j];
+                    }
+                    if (key0 + KEYS > sure) {                            // what the row does not see is minus infinity
+                        const int o = key0 - old, there = length - key0, n = limit - key0;      // the first key among the new rows; keys there are; keys seen
+                        unsigned long long seen = n >= KEYS ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1);
+                        if (masked && o > -KEYS && o < 64) seen |= (o >= 0 ? bits >> o : bits << -o) & (there >= KEYS ? ~0ull : (there <= 0 ? 0ull : (1ull << there) - 1));
 #pragma unroll
-                            for (int j = 0; j < HALF; j++)
-                                if (!((seen >> j) & 1)) a[j] = -INFINITY;
-                        }
-                    };
-                    float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    auto highest = [&]() {
+                        for (int j = 0; j < KEYS; j++)
+                            if (!((seen >> j) & 1)) a[j] = -INFINITY;
+                    }
+                    float x[4];
 #pragma unroll
-                        for (int j = 0; j < HALF; j += 8) {
+                    for (int e = 0; e < 4; e++) x[e] = max3(a[e], a[e + 4], a[e + 8]);
 #pragma unroll
-                            for (int e = 0; e < 4; e++) x[e] = max3(x[e], a[j + e], a[j + 4 + e]);
-                        }
-                    };
-                    scores(0);
-                    highest();
-                    scores(1);
-                    highest();
+                    for (int j = 12; j + 8 <= KEYS; j += 8) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[e] = max3(x[e], a[j + e], a[j + 4 + e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] = fmaxf(x[e], a[KEYS - 4 + e]);
                     float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * p.scale_log2;
                     s_part[s][blocks & 1][part][r] = top;
                     row_sync();
@@ -622,25 +640,21 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
                     const float ref = m == -INFINITY ? 0.f : -m;
                     const bool rescale = __any_sync(0xffffffffu, grown && valid) && kb > c.kb;      // (the same in the rows' other warp)
                     float more[4] = {0.f, 0.f, 0.f, 0.f};
-                    auto weights = [&](int h) {                          // -> the beginning of the scores, which have been read
-                        uint32_t pk[HALF / 2];
+                    // The weights go to the beginning of the part's scores, which have been read.
 #pragma unroll
-                        for (int j = 0; j < HALF; j += 2) {
-                            float e0 = a[j], e1 = a[j + 1];
+                    for (int h = 0; h < KEYS; h += 32) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            float e0 = a[h + j], e1 = a[h + j + 1];
                             fma2(e0, e1, p.scale_log2, ref);
                             e0 = exp2_approx(e0);
                             e1 = exp2_approx(e1);
                             add2(more[j & 2], more[(j & 2) + 1], e0, e1);
                             pk[j / 2] = pack2(e0, e1, (T*)nullptr);
                         }
-                        tmem_st16(tS + h * (HALF / 2), pk);
-                    };
-                    // (read again: 64 more registers are not there.  The second half's weights go behind the first's, 16 to 31 of the 64 columns: its own
-                    // scores begin at 32)
-                    scores(0);
-                    weights(0);
-                    scores(1);
-                    weights(1);
+                        tmem_st16(tS + h / 2, pk);
+                    }
                     sum[0] = sum[0] * al + (more[0] + more[2]);
                     sum[1] = sum[1] * al + (more[1] + more[3]);
                     if (rescale) {
@@ -705,7 +719,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
 #pragma unroll 1
             while (c.w < c.end) {
                 run(c, pair);
-                advance(c, p, l, s_req, pair);
+                advance(c, p, s_req, pair);
             }
         }
     }
@@ -734,7 +748,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
         hi = min(hi, lo + step);
     }
     const Request q = request_of(p, lo);
-    const Line l = line_of(p, p.plan[p.requests]);
+    const Line& l = p.line;
+    const Share single(l.odd + p.plan[p.requests], 2 * ctas);
     const int hk = head / p.group, g = head - hk * p.group, hs = g / p.tile_heads, in = g - hs * p.tile_heads;
     const long long row = (long long)t * p.heads + head, all = (long long)p.tokens * p.heads;
     // The row's two segments: their first pieces by row, the others by worker (`more`: of which array, rows of a worker, row in them).
@@ -748,7 +763,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
         const int ts = t / p.tile_tokens, tile = ts * p.head_sets + hs, r = (t - ts * p.tile_tokens) * p.tile_heads + in;
         const bool pair = tile < 2 * l.pairs;
         Segment& x = seg[0];
-        const Share share(pair ? l.pair_total : l.total, pair ? ctas : 2 * ctas);
+        const Share share = pair ? l.pair : single;
         const int start = pair ? (hk * l.pairs + tile / 2) * l.nbp : hk * l.nbp;
         x.from = x.to = -1;
         if (l.nbp > 0) {
@@ -765,7 +780,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     {
         const int dt = t - q.start, ts = dt / p.tile_tokens, tile = ts * p.head_sets + hs, r = (dt - ts * p.tile_tokens) * p.tile_heads + in;
         Segment& x = seg[1];
-        const Share share(l.total, 2 * ctas);
+        const Share& share = single;
         const int start = l.odd + p.plan[lo] + (tile * p.kv_heads + hk) * q.blocks;
         x.from = x.to = -1;
         if (q.blocks > 0) {
@@ -945,7 +960,14 @@ int b200_paged_attention(const b200_paged* c, const void* q, long long q_token, 
     p.table = c->page_table; p.lengths = c->lengths; p.row_starts = c->row_starts; p.prefix_pages = prefix_pages; p.mask = mask; p.out = out;
     p.table_stride = c->table_stride; p.out_token = out_token; p.out_head = out_head;
     p.requests = c->requests; p.tokens = c->tokens; p.heads = c->heads; p.kv_heads = c->kv_heads;
-    p.page_size = c->page_size; p.box_rows = box; p.table_width = c->table_width; p.prefix = prefix_length;
+    p.page_size = c->page_size; p.page_blocks = c->page_size / kKeys; p.box_rows = box;
+    while (1 << p.page_shift < c->page_size) p.page_shift++;
+    p.line.nbp = (prefix_length + kKeys - 1) / kKeys;
+    p.line.tiles = (c->tokens + p.tile_tokens - 1) / p.tile_tokens * p.head_sets;
+    p.line.pairs = p.line.tiles / 2;
+    p.line.odd = p.line.tiles & 1 ? c->kv_heads * p.line.nbp : 0;
+    p.line.pair = Share(c->kv_heads * p.line.pairs * p.line.nbp, ctas);
+    p.table_width = c->table_width; p.prefix = prefix_length;
     // (of a scale of nothing, weights are equal; a positive one, however small, keeps hidden scores at minus infinity)
     p.negative = scale < 0.f;
     p.scale_log2 = std::max(std::abs(scale) * 1.4426950408889634f, 1e-30f);
