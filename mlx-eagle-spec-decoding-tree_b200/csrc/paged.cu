@@ -731,13 +731,15 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
     }
 }
 
-// A warp joins the pieces of one query row: a lane looks at a piece's statistics, then all lanes add its output, four dims (two) each.
-template <typename T, int HD>
+// A warp joins the pieces of one query row: a lane looks at a piece's statistics, then all lanes add its output, four dims (two) each.  With WAYS
+// of 4 a row has the four warps of a CTA, every fourth piece each: where there are few rows, they have many pieces, and too few warps to have
+// their loads in flight.
+template <typename T, int HD, int WAYS>
 __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedParams p, int ctas) {
     pdl_launch_dependents();
     pdl_wait();
     constexpr int N = HD / 32, BATCH = 4;
-    const int lane = threadIdx.x & 31, head = blockIdx.y * 4 + (threadIdx.x >> 5), t = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = WAYS == 1 ? blockIdx.y * 4 + warp : blockIdx.y, t = blockIdx.x, way = WAYS == 1 ? 0 : warp;
     if (head >= p.heads) return;
     if (t < p.row_starts[0] || t >= p.row_starts[p.requests]) return;
     int lo = 0, hi = p.requests;
@@ -797,9 +799,9 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     const int n0 = seg[0].from < 0 ? 0 : seg[0].to - seg[0].from + 1, n = n0 + (seg[1].from < 0 ? 0 : seg[1].to - seg[1].from + 1);
     float m = -INFINITY, sum = 0.f, o[N] = {};
 #pragma unroll 1
-    for (int base = 0; base < n; base += 32) {
+    for (int base = 0; base < n; base += 32 * WAYS) {
         // a piece a lane
-        const int k = base + lane;
+        const int k = base + lane * WAYS + way;
         const float* src = nullptr;
         float2 x = make_float2(-INFINITY, 0.f);
         if (k < n) {
@@ -817,7 +819,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
         float top = x.x;
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        if (top == -INFINITY) continue;
+        if (top == -INFINITY) continue;                                  // (the same in all lanes)
         const float high = fmaxf(m, top), before = exp2_approx(m - high), weight = x.x == -INFINITY ? 0.f : exp2_approx(x.x - high);
         float l2 = weight * x.y;
 #pragma unroll
@@ -846,6 +848,29 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
             for (int b = 0; b < BATCH; b++)
 #pragma unroll
                 for (int e = 0; e < N; e++) o[e] += w[b] * v[b].v[e];
+        }
+    }
+    if constexpr (WAYS > 1) {
+        __shared__ float s_m[WAYS], s_sum[WAYS], s_o[WAYS][HD];
+        if (lane == 0) {
+            s_m[way] = m;
+            s_sum[way] = sum;
+        }
+#pragma unroll
+        for (int e = 0; e < N; e++) s_o[way][lane * N + e] = o[e];
+        __syncthreads();
+        if (way > 0) return;
+        m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+        sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < N; e++) o[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAYS; w++) {                                 // (in order: the same bits every time)
+            if (s_m[w] == -INFINITY) continue;
+            const float a = exp2_approx(s_m[w] - m);
+            sum += a * s_sum[w];
+#pragma unroll
+            for (int e = 0; e < N; e++) o[e] += a * s_o[w][lane * N + e];
         }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -888,7 +913,9 @@ int launch_paged(const PagedParams& p, int ctas, cudaStream_t stream) {
     if (!allow_smem(kern, PGeo<HD>::SMEM, done)) return check_launch();
     const int rc = launch_chain(kern, dim3(ctas), kPgThreads, PGeo<HD>::SMEM, 1, stream, p);
     if (rc != B200_OK) return rc;
-    launch_kernel(paged_join_kernel<T, HD>, dim3(p.tokens, (p.heads + 3) / 4), dim3(128), 0, stream, p, ctas);
+    // (a row a CTA as long as its warps find room at once)
+    if ((long long)p.tokens * p.heads <= 16 * ctas) launch_kernel(paged_join_kernel<T, HD, 4>, dim3(p.tokens, p.heads), dim3(128), 0, stream, p, ctas);
+    else launch_kernel(paged_join_kernel<T, HD, 1>, dim3(p.tokens, (p.heads + 3) / 4), dim3(128), 0, stream, p, ctas);
     return check_launch();
 }
 
