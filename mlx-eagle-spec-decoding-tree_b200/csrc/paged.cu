@@ -46,18 +46,25 @@ struct PGeo {
 // A line of blocks dealt out to workers in equal stretches, none of them empty: n of them, the first r of q + 1 blocks, the others of q.
 struct Share {
     int total, n, q, r;
-    __host__ __device__ Share() {}
-    __host__ __device__ __forceinline__ Share(int total, int workers)
-        : total(total), n(workers < total ? workers : total), q(n ? total / n : 0), r(total - q * n) {}
+    __device__ __forceinline__ Share(int total, int workers) : total(total), n(min(workers, total)), q(n ? total / n : 0), r(total - q * n) {}
     __device__ __forceinline__ int start(int w) const { return w < n ? q * w + min(w, r) : total; }
     __device__ __forceinline__ int owner(int b) const { return b < r * (q + 1) ? b / (q + 1) : r + (b - r * (q + 1)) / q; }
 };
-// Blocks of the prefix, its query tiles (per kv head) and pairs of them; its blocks for tiles without a partner, which head the line of
-// single streams; the line of pairs and its workers.
+// Blocks of the prefix, its query tiles (per kv head) and pairs of them, blocks for pairs; blocks for tiles without a partner, which head the
+// line of single streams.
 struct Line {
-    int nbp, tiles, pairs, odd;
-    Share pair;
+    int nbp, tiles, pairs, pair_total, odd;
 };
+// CTAs for single streams, of `ctas`: each has either pairs or single streams, so that a CTA leaves two pieces, not four, and never changes from
+// the one to the other (12000 cycles).  By the time they take, in units of 2100 cycles: 2 a block of a pair, 1 a block of single streams, which
+// run side by side, and 2 more a segment of theirs.
+__device__ __forceinline__ int single_ctas(const Line& l, int own, int segments, int kv_heads, int ctas) {
+    const int single = l.odd + own;
+    if (l.pair_total == 0) return ctas;
+    if (single == 0) return 0;
+    const float a = 2.f * l.pair_total, b = (float)single + 2.f * (segments + (l.odd ? kv_heads : 0));
+    return min(max((int)(b / (a + b) * ctas + 0.5f), 1), ctas - 1);
+}
 
 struct PagedParams {
     CUtensorMap qmap, qhmap, q1map, kmap, vmap;  // queries by tile, half a tile and token; pages
@@ -66,7 +73,7 @@ struct PagedParams {
     void* out;
     float *first_prefix, *first_own, *more_pair, *more;      // pieces [..][HD]
     float2* ml;                                  // (m, l) in the order of the pieces
-    int* plan;                                   // sums of the own blocks, by request
+    int* plan;                                   // sums of the own blocks, by request; CTAs for single streams
     long long table_stride, out_token, out_head;
     int requests, tokens, heads, kv_heads, group, tile_heads, tile_tokens, half_tokens, head_sets;
     int page_size, page_shift, page_blocks;      // a page's rows; their logarithm, or the page's blocks if it is more than one
@@ -246,12 +253,14 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
     __shared__ int s_cum[kPgMaxRequests + 1];
     __shared__ Request s_req[kPgMaxRequests];
     __shared__ long long s_warp[kPgThreads / 32];
-    __shared__ Cursor s_from[3];                                         // of the pairs, of either stream
+    __shared__ Cursor s_from[2];                                         // of either stream; the first's for both of a pair
+    __shared__ int s_segments;
     __shared__ float s_part[2][2][kParts][kRows];                        // [stream][in turn]: what a row's threads tell one another
     const uint32_t sbase = smem_u32(smem);
     const int lane = threadIdx.x & 31, warp = uniform(threadIdx.x >> 5), ctas = gridDim.x, cta = blockIdx.x;
 
     if (threadIdx.x == 0) {
+        s_segments = 0;
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(&p.kmap) : "memory");
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(&p.vmap) : "memory");
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(&p.qmap) : "memory");
@@ -290,11 +299,15 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
     {
         const int per = (p.requests + kPgThreads - 1) / kPgThreads, b0 = min((int)threadIdx.x * per, p.requests), b1 = min(b0 + per, p.requests);
         long long mine = 0, before;
+        int segments = 0;
         for (int b = b0; b < b1; b++) {
             const Request r = request_of(p, b);
             s_req[b] = r;
             mine += (long long)r.blocks * r.tiles * p.kv_heads;
+            if (r.blocks > 0) segments += r.tiles * p.kv_heads;
         }
+        segments = __reduce_add_sync(0xffffffffu, segments);
+        if (lane == 0 && segments > 0) atomicAdd(&s_segments, segments);
         long long scan = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -312,19 +325,20 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
         if (threadIdx.x == kPgThreads - 1) s_cum[p.requests] = (int)min(before, 1ll << 28);
         __syncthreads();
     }
-    if (warp < 3 && lane == 0) {
+    const int singles = uniform(single_ctas(p.line, s_cum[p.requests], s_segments, p.kv_heads, ctas));
+    const bool pair = cta < ctas - singles;
+    if (warp < 2 && lane == 0) {
         // (the streams' workers: first one of every CTA, then the other)
-        const bool pair = warp == 0;
-        const Share share = pair ? p.line.pair : Share(p.line.odd + s_cum[p.requests], 2 * ctas);
-        const int w = cta + (warp == 2 ? ctas : 0);
+        const Share share = pair ? Share(p.line.pair_total, ctas - singles) : Share(p.line.odd + s_cum[p.requests], 2 * singles);
+        const int w = pair ? cta : cta - (ctas - singles) + warp * singles;
         s_from[warp] = cursor_at(p, s_cum, s_req, pair, share.start(w), share.start(w + 1));
-    } else if (cta == 0 && warp >= 3) {
-        for (int b = threadIdx.x - 96; b <= p.requests; b += kPgThreads - 96) p.plan[b] = s_cum[b];
+    } else if (cta == 0 && warp >= 2) {
+        for (int b = threadIdx.x - 64; b <= p.requests; b += kPgThreads - 64) p.plan[b] = s_cum[b];
+        if (threadIdx.x == 64) p.plan[p.requests + 1] = singles;
     }
     __syncthreads();
-    // Blocks of pairs, of either stream.  Every other CTA begins with the latter: pairs keep the tensor cores busy, the rest the memory.
-    const int turn = cta & 1;
-    const int np = uniform(s_from[0].end - s_from[0].w), n0 = uniform(s_from[1].end - s_from[1].w), n1 = uniform(s_from[2].end - s_from[2].w);
+    // Blocks of either stream (a pair's are the same).
+    const int n0 = uniform(s_from[0].end - s_from[0].w), n1 = uniform(s_from[1].end - s_from[1].w);
 
     if (warp == kLoader) {
         // ------------------------------------------------------------------ keys, queries and values, in the order of their use
@@ -420,36 +434,24 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
                 x.ahead = page_at(x, x.kb);
             }
         };
+        At x, y;
+        if (n0 > 0) {
+            start(x, 0);
+            keys(x, pair ? 2 : 0);
+        }
+        if (!pair && n1 > 0) {
+            start(y, 1);
+            keys(y, 1);
+        }
 #pragma unroll 1
-        for (int phase = 0; phase < 2; phase++) {
-            At x, y;
-            if (phase == turn) {
-                if (np > 0) start(x, 0);
-#pragma unroll 1
-                for (int i = 0; i < np; i++) {
-                    keys(x, 2);
-                    values(x);
-                }
-            } else {
-                if (n0 > 0) {
-                    start(x, 1);
-                    keys(x, 0);
-                }
-                if (n1 > 0) {
-                    start(y, 2);
-                    keys(y, 1);
-                }
-#pragma unroll 1
-                for (int i = 0; i < max(n0, n1); i++) {
-                    if (i < n0) {
-                        values(x);
-                        if (i + 1 < n0) keys(x, 0);
-                    }
-                    if (i < n1) {
-                        values(y);
-                        if (i + 1 < n1) keys(y, 1);
-                    }
-                }
+        for (int i = 0; i < max(n0, n1); i++) {
+            if (i < n0) {
+                values(x);
+                if (i + 1 < n0) keys(x, pair ? 2 : 0);
+            }
+            if (!pair && i < n1) {
+                values(y);
+                if (i + 1 < n1) keys(y, 1);
             }
         }
     } else if (warp == kIssuer) {
@@ -460,7 +462,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
         const uint64_t qdesc = sw128_desc(sbase), kdesc = sw128_desc(sbase + G::KV0), vdesc = sw128_desc_n_major(sbase + G::KV0 + ST * G::SLOT, kKeys * 128);
         struct At {
             Cursor c;
-            int left;                                                    // blocks of the phase whose scores have not been asked for
+            int left;                                                    // blocks whose scores have not been asked for
             int kb, kb1;                                                 // of the piece
             int keys;                                                    // of the block whose scores were asked for last
             bool first, small;                                           // ... of its piece; its queries take half a tile
@@ -468,7 +470,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
         } at[2];
         int kring = 0, vring = 0;
         // Scores of the next block of stream s.  take: wait for its keys, give: hand them back (a pair's second stream does).
-        auto scores = [&](int s, At& x, bool pair, bool take, bool give) {
+        auto scores = [&](int s, At& x, bool take, bool give) {
             const int slot = kring % ST;
             x.first = x.kb == x.kb1;
             if (x.first) {
@@ -546,29 +548,21 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
         for (int s = 0; s < 2; s++) {
             at[s].blocks = at[s].came0 = at[s].came1 = 0;
             at[s].half = 1;
+            at[s].c = s_from[pair ? 0 : s];
+            at[s].left = s ? n1 : n0;
+            at[s].kb = at[s].kb1 = 0;
         }
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+            if (at[s].left > 0) scores(s, at[s], !pair || s == 0, !pair || s == 1);
 #pragma unroll 1
-        for (int phase = 0; phase < 2; phase++) {
-            const bool pair = phase == turn;
+        for (int i = 0; i < max(n0, n1); i++)
 #pragma unroll
             for (int s = 0; s < 2; s++) {
-                at[s].c = s_from[pair ? 0 : 1 + s];
-                at[s].left = pair ? np : (s ? n1 : n0);
-                at[s].kb = at[s].kb1 = 0;
+                if (i >= (s ? n1 : n0)) continue;
+                output(s, at[s], !pair || s == 0, !pair || s == 1);
+                if (at[s].left > 0) scores(s, at[s], !pair || s == 0, !pair || s == 1);
             }
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-                if (at[s].left > 0) scores(s, at[s], pair, !pair || s == 0, !pair || s == 1);
-            const int most = pair ? np : max(n0, n1);
-#pragma unroll 1
-            for (int i = 0; i < most; i++)
-#pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    if (i >= (pair ? np : (s ? n1 : n0))) continue;
-                    output(s, at[s], !pair || s == 0, !pair || s == 1);
-                    if (at[s].left > 0) scores(s, at[s], pair, !pair || s == 0, !pair || s == 1);
-                }
-        }
     } else {
         // ------------------------------------------------------------------ softmax: 64 keys of a block of a query row a thread
         constexpr int KEYS = kKeys / kParts, DIMS = HD / kParts;
@@ -578,7 +572,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
         const int dt = r / p.tile_heads;
         auto row_sync = [&]() { asm volatile("bar.sync %0, %1;\n" ::"r"(1 + s * 4 + (warp & 3)), "n"(kParts * 32) : "memory"); };      // the warps of these rows
         int blocks = 0;
-        auto run = [&](const Cursor& c, bool pair) {
+        auto run = [&](const Cursor& c) {
             const Tile tile = tile_of(p, c.r, c.tile + (pair ? s : 0));
             const int rows = tile.toks * p.tile_heads, g = tile.hs * p.tile_heads + r - dt * p.tile_heads, t = tile.tok0 + dt, kb1 = c.last();
             const bool valid = dt < tile.toks && g < p.group, busy = (warp & 3) * 32 < rows;      // (busy: some row of the warp may be)
@@ -692,35 +686,52 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
                     at = (c.req < 0 ? 0 : all) + row;
                 } else {
                     // (pairs: 256 rows a CTA; single streams: 128 a stream, behind them)
-                    const long long slot = pair ? (long long)cta * 2 * kRows + s * kRows + r : ((long long)s * ctas + cta) * kRows + r;
+                    const int w = cta - (ctas - singles) + s * singles;          // (of single streams)
+                    const long long slot = pair ? (long long)cta * 2 * kRows + s * kRows + r : (long long)w * kRows + r;
                     dst = (pair ? p.more_pair : p.more) + slot * HD;
                     at = 2 * all + (pair ? 0 : (long long)ctas * 2 * kRows) + slot;
                 }
                 if (valid && part == 0) p.ml[at] = make_float2(l == l ? m : INFINITY, l);      // (scores of NaN alone leave no maximum, but the row is NaN)
+                // Rows of four lanes at a time: each takes a quarter of the 32 dims of all four, so that a store covers whole lines of memory.  (A row a
+                // lane: 3300 cycles, 7000 with both streams at it.)
+                const unsigned long long mine = reinterpret_cast<unsigned long long>(dst + part * DIMS);      // (used where the row is valid)
 #pragma unroll
                 for (int d = 0; d < DIMS; d += 32) {
                     uint32_t o[32];
                     tmem_ld32(o, tO + d);
                     asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-                    if (valid) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 8)                  // (whole sectors: halves of them took twice as long)
-                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(dst + part * DIMS + d + j), "r"(o[j]), "r"(o[j + 1]),
-                                         "r"(o[j + 2]), "r"(o[j + 3]), "r"(o[j + 4]), "r"(o[j + 5]), "r"(o[j + 6]), "r"(o[j + 7]) : "memory");
+                    for (int x = 1; x < 4; x *= 2) {
+#pragma unroll
+                        for (int a = 0; a < 4; a++) {
+                            if (a & x) continue;
+#pragma unroll
+                            for (int j = 0; j < 8; j++) {
+                                uint32_t &lo = o[a * 8 + j], &hi = o[(a | x) * 8 + j];
+                                const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & x ? lo : hi, x);
+                                if (lane & x) lo = other;
+                                else hi = other;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int a = 0; a < 4; a++) {                        // unit `lane & 3` of the row of lane a of the four
+                        const unsigned long long to = __shfl_sync(0xffffffffu, mine, (lane & ~3) | a) + (lane & 3) * 32 + d * 4;
+                        const bool there = __shfl_sync(0xffffffffu, (int)valid, (lane & ~3) | a);
+                        const uint32_t* v = o + a * 8;
+                        if (there)
+                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                                         "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
                     }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
             }
         };
+        Cursor c = s_from[pair ? 0 : s];
 #pragma unroll 1
-        for (int phase = 0; phase < 2; phase++) {
-            const bool pair = phase == turn;
-            Cursor c = s_from[pair ? 0 : 1 + s];
-#pragma unroll 1
-            while (c.w < c.end) {
-                run(c, pair);
-                advance(c, p, s_req, pair);
-            }
+        while (c.w < c.end) {
+            run(c);
+            advance(c, p, s_req, pair);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
@@ -751,7 +762,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     }
     const Request q = request_of(p, lo);
     const Line& l = p.line;
-    const Share single(l.odd + p.plan[p.requests], 2 * ctas);
+    const int singles = p.plan[p.requests + 1];
+    const Share single(l.odd + p.plan[p.requests], 2 * singles);
     const int hk = head / p.group, g = head - hk * p.group, hs = g / p.tile_heads, in = g - hs * p.tile_heads;
     const long long row = (long long)t * p.heads + head, all = (long long)p.tokens * p.heads;
     // The row's two segments: their first pieces by row, the others by worker (`more`: of which array, rows of a worker, row in them).
@@ -765,7 +777,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
         const int ts = t / p.tile_tokens, tile = ts * p.head_sets + hs, r = (t - ts * p.tile_tokens) * p.tile_heads + in;
         const bool pair = tile < 2 * l.pairs;
         Segment& x = seg[0];
-        const Share share = pair ? l.pair : single;
+        const Share share = pair ? Share(l.pair_total, ctas - singles) : single;
         const int start = pair ? (hk * l.pairs + tile / 2) * l.nbp : hk * l.nbp;
         x.from = x.to = -1;
         if (l.nbp > 0) {
@@ -893,7 +905,7 @@ Room room_of(const b200_paged* c, int ctas) {
     r.more = r.pair + pair * row;
     r.ml = r.more + more * row;
     r.plan = r.ml + (2 * all + pair + more) * sizeof(float2);
-    r.total = r.plan + (c->requests + 1) * sizeof(int);
+    r.total = r.plan + (c->requests + 2) * sizeof(int);
     r.total = (r.total + 15) / 16 * 16;
     return r;
 }
@@ -993,7 +1005,7 @@ int b200_paged_attention(const b200_paged* c, const void* q, long long q_token, 
     p.line.tiles = (c->tokens + p.tile_tokens - 1) / p.tile_tokens * p.head_sets;
     p.line.pairs = p.line.tiles / 2;
     p.line.odd = p.line.tiles & 1 ? c->kv_heads * p.line.nbp : 0;
-    p.line.pair = Share(c->kv_heads * p.line.pairs * p.line.nbp, ctas);
+    p.line.pair_total = c->kv_heads * p.line.pairs * p.line.nbp;
     p.table_width = c->table_width; p.prefix = prefix_length;
     // (of a scale of nothing, weights are equal; a positive one, however small, keeps hidden scores at minus infinity)
     p.negative = scale < 0.f;
