@@ -31,9 +31,9 @@ namespace {
 constexpr int kKeys = 128;                       // of a block
 constexpr int kRows = 128;                       // query rows of a tile
 constexpr int kParts = 2;                        // threads of a query row
-constexpr int kPgThreads = 576;                  // 2 x 8 softmax warps, copies, products: few enough for 112 registers a thread
+constexpr int kPgThreads = 608;                  // 2 x 8 softmax warps, keys and queries, products, values
 constexpr int kPgMaxRequests = 1024;
-constexpr int kLoader = 16, kIssuer = 17;
+constexpr int kKeyLoader = 16, kIssuer = 17, kValueLoader = 18;
 constexpr float kLag = 8.f;                      // a row's maximum may exceed its reference by 2^8
 
 template <int HD>
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
     pdl_launch_dependents();
     pdl_wait();
     // (what earlier kernels wrote by ordinary stores, rows and queries: 2000 cycles, of which all but a few pass behind the scan below)
-    if (warp == kLoader) asm volatile("fence.proxy.async;\n" ::: "memory");
+    if (warp == kKeyLoader || warp == kValueLoader) asm volatile("fence.proxy.async;\n" ::: "memory");
 
     // ---- own blocks ahead of each request: consecutive requests a thread, then a scan (a line beyond 2^28 blocks is cut there)
     {
@@ -340,9 +340,14 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
     // Blocks of either stream (a pair's are the same).
     const int n0 = uniform(s_from[0].end - s_from[0].w), n1 = uniform(s_from[1].end - s_from[1].w);
 
-    if (warp == kLoader) {
-        // ------------------------------------------------------------------ keys, queries and values, in the order of their use
-        int kring = 0, vring = 0;
+    if (warp == kKeyLoader || warp == kValueLoader) {
+        // ------------------------------------------------------------------ keys and queries, or values, in the order of their use
+        // (both by one warp: 73 us in place of 64 for the 64 requests of the benchmark in pages of 16, eight boxes a tile and 64 dims)
+        const bool values = warp == kValueLoader;
+        const CUtensorMap* map = values ? &p.vmap : &p.kmap;
+        uint64_t *const full = values ? vfull : kfull, *const free = values ? vfree : kfree;
+        const uint32_t slots = sbase + G::KV0 + (values ? ST * G::SLOT : 0);
+        int ring = 0;
         int asked[4] = {0, 0, 0, 0}, half = 3;                           // uses of the streams' halves of queries; the halves last taken, a bit a stream
         // A tile of queries, or, of 64 rows at most, one of its halves in turn, so that the next piece's come while this one's are in use.
         auto ask = [&](int s, const Cursor& c, int tile) {
@@ -377,8 +382,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
         struct At {
             Cursor c;
             int kb, kb1;                                                 // of the piece
-            int page, ahead;                                             // pages a lane: of the block whose keys came last, of the next
-            int boxes, row, hk;                                          // ... its boxes, first row in its page, head
+            int ahead;                                                   // a page of the next block a lane
         };
         auto page_at = [&](const At& x, int kb) {
             const int key = kb * kKeys + (lane & 15) * p.box_rows;
@@ -395,35 +399,23 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
             x.kb1 = x.c.last();
             x.ahead = page_at(x, x.kb);
         };
-        auto copy = [&](const At& x, const CUtensorMap* map, uint32_t bar, uint32_t dst) {
-            if (elect_one()) mbar_expect_tx(bar, x.boxes * p.box_rows * HD * 2);
+        // The cursor's next block; s: the stream that uses it, 2: both.
+        auto next = [&](At& x, int s) {
+            const bool first = x.kb == x.c.kb;
+            const int page = x.ahead, key0 = x.kb * kKeys, slot = ring % ST, row = p.page_blocks > 1 ? x.kb % p.page_blocks * kKeys : 0;
+            const int boxes = (min(kKeys, x.c.r.length - key0) + p.box_rows - 1) / p.box_rows;
+            x.ahead = page_at(x, x.kb + 1);
+            if (ring >= ST) mbar_wait_reported(smem_u32(free + slot), (ring / ST - 1) & 1, p.polls, p.err, 31);
+            __syncwarp();
+            const uint32_t bar = smem_u32(full + slot), dst = slots + slot * G::SLOT;
+            if (elect_one()) mbar_expect_tx(bar, boxes * p.box_rows * HD * 2);
             __syncwarp();
             // (a box a lane, a page's next 64 dims in the lanes behind: from one thread, one after the other, they took half as long again)
-            if ((lane & 15) < x.boxes && lane >> 4 < NB)
-                tma_box4(dst + (lane >> 4) * (kKeys * 128) + (lane & 15) * p.box_rows * 128, map, (lane >> 4) * 64, x.row, x.hk, x.page, bar);
+            if ((lane & 15) < boxes && lane >> 4 < NB)
+                tma_box4(dst + (lane >> 4) * (kKeys * 128) + (lane & 15) * p.box_rows * 128, map, (lane >> 4) * 64, row, x.c.hk, page, bar);
             __syncwarp();
-        };
-        auto values = [&](At& x) {                                       // of the block whose keys came last
-            const int slot = vring % ST;
-            if (vring >= ST) mbar_wait_reported(smem_u32(vfree + slot), (vring / ST - 1) & 1, p.polls, p.err, 31);
-            __syncwarp();
-            copy(x, &p.vmap, smem_u32(vfull + slot), sbase + G::KV0 + (ST + slot) * G::SLOT);
-            vring++;
-        };
-        // Keys of the cursor's next block, and the queries of its piece; s: the stream that uses it, 2: both.
-        auto keys = [&](At& x, int s) {
-            const bool first = x.kb == x.c.kb;
-            const int key0 = x.kb * kKeys, slot = kring % ST;
-            x.page = x.ahead;
-            x.row = p.page_blocks > 1 ? x.kb % p.page_blocks * kKeys : 0;
-            x.hk = x.c.hk;
-            x.boxes = (min(kKeys, x.c.r.length - key0) + p.box_rows - 1) / p.box_rows;
-            x.ahead = page_at(x, x.kb + 1);
-            if (kring >= ST) mbar_wait_reported(smem_u32(kfree + slot), (kring / ST - 1) & 1, p.polls, p.err, 31);
-            __syncwarp();
-            copy(x, &p.kmap, smem_u32(kfull + slot), sbase + G::KV0 + slot * G::SLOT);
-            kring++;
-            if (first) {                                                 // (behind the keys: their slot is free earlier)
+            ring++;
+            if (first && !values) {                                      // (behind the keys: their slot is free earlier)
                 if (s != 1) ask(0, x.c, x.c.tile);
                 if (s != 0) ask(1, x.c, x.c.tile + (s == 2));
             }
@@ -435,24 +427,12 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
             }
         };
         At x, y;
-        if (n0 > 0) {
-            start(x, 0);
-            keys(x, pair ? 2 : 0);
-        }
-        if (!pair && n1 > 0) {
-            start(y, 1);
-            keys(y, 1);
-        }
+        if (n0 > 0) start(x, 0);
+        if (!pair && n1 > 0) start(y, 1);
 #pragma unroll 1
         for (int i = 0; i < max(n0, n1); i++) {
-            if (i < n0) {
-                values(x);
-                if (i + 1 < n0) keys(x, pair ? 2 : 0);
-            }
-            if (!pair && i < n1) {
-                values(y);
-                if (i + 1 < n1) keys(y, 1);
-            }
+            if (i < n0) next(x, pair ? 2 : 0);
+            if (!pair && i < n1) next(y, 1);
         }
     } else if (warp == kIssuer) {
         // ------------------------------------------------------------------ products
@@ -692,35 +672,42 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
                     at = 2 * all + (pair ? 0 : (long long)ctas * 2 * kRows) + slot;
                 }
                 if (valid && part == 0) p.ml[at] = make_float2(l == l ? m : INFINITY, l);      // (scores of NaN alone leave no maximum, but the row is NaN)
-                // Rows of four lanes at a time: each takes a quarter of the 32 dims of all four, so that a store covers whole lines of memory.  (A row a
-                // lane: 3300 cycles, 7000 with both streams at it.)
                 const unsigned long long mine = reinterpret_cast<unsigned long long>(dst + part * DIMS);      // (used where the row is valid)
+                const bool many = rows > 16;
 #pragma unroll
                 for (int d = 0; d < DIMS; d += 32) {
                     uint32_t o[32];
                     tmem_ld32(o, tO + d);
                     asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+                    if (many) {
+                        // Rows of four lanes at a time: each takes a quarter of the 32 dims of all four, so that a store covers whole lines of memory.  (A row
+                        // a lane: 3300 cycles, 7000 with both streams at it.)
 #pragma unroll
-                    for (int x = 1; x < 4; x *= 2) {
+                        for (int x = 1; x < 4; x *= 2) {
 #pragma unroll
-                        for (int a = 0; a < 4; a++) {
-                            if (a & x) continue;
+                            for (int a = 0; a < 4; a++) {
+                                if (a & x) continue;
 #pragma unroll
-                            for (int j = 0; j < 8; j++) {
-                                uint32_t &lo = o[a * 8 + j], &hi = o[(a | x) * 8 + j];
-                                const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & x ? lo : hi, x);
-                                if (lane & x) lo = other;
-                                else hi = other;
+                                for (int j = 0; j < 8; j++) {
+                                    uint32_t &lo = o[a * 8 + j], &hi = o[(a | x) * 8 + j];
+                                    const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & x ? lo : hi, x);
+                                    if (lane & x) lo = other;
+                                    else hi = other;
+                                }
                             }
                         }
                     }
 #pragma unroll
-                    for (int a = 0; a < 4; a++) {                        // unit `lane & 3` of the row of lane a of the four
-                        const unsigned long long to = __shfl_sync(0xffffffffu, mine, (lane & ~3) | a) + (lane & 3) * 32 + d * 4;
-                        const bool there = __shfl_sync(0xffffffffu, (int)valid, (lane & ~3) | a);
+                    for (int a = 0; a < 4; a++) {                        // unit `lane & 3` of the row of lane a of the four; or unit a of the own row
+                        unsigned long long to = mine + a * 32;
+                        bool there = valid;
+                        if (many) {
+                            to = __shfl_sync(0xffffffffu, mine, (lane & ~3) | a) + (lane & 3) * 32;
+                            there = __shfl_sync(0xffffffffu, (int)valid, (lane & ~3) | a);
+                        }
                         const uint32_t* v = o + a * 8;
                         if (there)
-                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(to + d * 4), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
                                          "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
                     }
                 }
