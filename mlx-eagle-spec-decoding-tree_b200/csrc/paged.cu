@@ -55,6 +55,14 @@ struct Share {
 struct Line {
     int nbp, tiles, pairs, pair_total, odd;
 };
+// Blocks of a pair's segment that come first, for all pairs of a head, then what is left of them: a worker's stretch, so that all that work on a head
+// at a time stand at the same keys and find them in L2.  (Segment by segment, stretches of 222 blocks begin anywhere in the 256 of a prefix of
+// 32768 rows: 1.87 GB of its 134 MB were read from HBM for 16 pairs.)  Only where a stretch is more than half a segment.
+__device__ __forceinline__ int first_blocks(const Line& l, int workers) {
+    if (l.pairs < 2 || workers < 1) return l.nbp;
+    const int stretch = (l.pair_total + workers - 1) / workers;
+    return stretch < l.nbp && l.nbp <= 2 * stretch ? stretch : l.nbp;
+}
 // CTAs for single streams, of `ctas`: each has either pairs or single streams, so that a CTA leaves two pieces, not four, and never changes from
 // the one to the other (12000 cycles).  By the time they take, in units of 2100 cycles: 2 a block of a pair, 1 a block of single streams, which
 // run side by side, and 2 more a segment of theirs.
@@ -71,7 +79,7 @@ struct PagedParams {
     const int *table, *lengths, *row_starts, *prefix_pages;
     const unsigned long long* mask;
     void* out;
-    float *first_prefix, *first_own, *more_pair, *more;      // pieces [..][HD]
+    float *first_prefix, *first_own, *first_behind, *more_pair, *more;      // pieces [..][HD]
     float2* ml;                                  // (m, l) in the order of the pieces
     int* plan;                                   // sums of the own blocks, by request; CTAs for single streams
     long long table_stride, out_token, out_head;
@@ -101,10 +109,11 @@ __device__ __forceinline__ Request request_of(const PagedParams& p, int b) {
     return r;
 }
 
-// A worker's place in the line: block kb of `blocks` of a segment.
+// A worker's place in the line: block kb of a segment that ends before `blocks`.
 struct Cursor {
     int w, end;                                  // in the line
     int kb, blocks;
+    int head;                                    // where the segment begins: 0, or behind the blocks of a pair that came first
     int req;                                     // -1: the prefix
     int hk, tile;
     Request r;                                   // of the prefix: all tokens, its rows
@@ -114,23 +123,33 @@ __device__ __forceinline__ void enter(Cursor& c, const Request* reqs, int req) {
     c.req = req;
     c.r = reqs[req];
     c.blocks = c.r.blocks;
-    c.tile = c.hk = c.kb = 0;
+    c.tile = c.hk = c.kb = c.head = 0;
 }
 // The cursor of block w of the line of pairs (its tile is the first stream's) or of single streams; cum: own blocks ahead of each request.
-__device__ __forceinline__ Cursor cursor_at(const PagedParams& p, const int* cum, const Request* reqs, bool pair, int w, int end) {
+// `ahead`: blocks of a pair's segment that come first.
+__device__ __forceinline__ Cursor cursor_at(const PagedParams& p, const int* cum, const Request* reqs, bool pair, int ahead, int w, int end) {
     const Line& l = p.line;
     Cursor c{};
     c.w = w;
     c.end = end;
     if (w >= end) return c;
     if (pair || w < l.odd) {
-        const int seg = w / l.nbp;
         c.req = -1;
         c.r = {0, p.tokens, p.prefix, p.prefix, l.nbp, l.tiles};
-        c.blocks = l.nbp;
-        c.kb = w - seg * l.nbp;
-        c.hk = pair ? seg / l.pairs : seg;
-        c.tile = pair ? 2 * (seg - c.hk * l.pairs) : l.tiles - 1;
+        int blocks = l.nbp, in = w;
+        if (pair) {
+            c.hk = w / (l.pairs * l.nbp);
+            in = w - c.hk * l.pairs * l.nbp;
+            const bool behind = in >= l.pairs * ahead;
+            if (behind) in -= l.pairs * ahead;
+            c.head = behind ? ahead : 0;
+            blocks = behind ? l.nbp - ahead : ahead;
+        }
+        const int seg = in / blocks;
+        c.kb = c.head + in - seg * blocks;
+        c.blocks = c.head + blocks;
+        if (pair) c.tile = 2 * seg;
+        else c.hk = seg, c.tile = l.tiles - 1;
         return c;
     }
     const int v = w - l.odd;
@@ -148,17 +167,20 @@ __device__ __forceinline__ Cursor cursor_at(const PagedParams& p, const int* cum
     return c;
 }
 // Past its piece.
-__device__ __forceinline__ void advance(Cursor& c, const PagedParams& p, const Request* reqs, bool pair) {
+__device__ __forceinline__ void advance(Cursor& c, const PagedParams& p, const Request* reqs, bool pair, int ahead) {
     const int n = c.last() - c.kb;
     c.w += n;
     c.kb += n;
     if (c.kb < c.blocks || c.w >= c.end) return;
-    c.kb = 0;
+    c.kb = c.head;
     if (pair) {
         c.tile += 2;
         if (c.tile < 2 * p.line.pairs) return;
         c.tile = 0;
-        c.hk++;
+        const bool behind = c.head == 0 && ahead < p.line.nbp;           // what is left of the head's segments, or the next head
+        if (!behind) c.hk++;
+        c.kb = c.head = behind ? ahead : 0;
+        c.blocks = behind ? p.line.nbp : ahead;
         return;
     }
     if (++c.hk < p.kv_heads) return;
@@ -227,21 +249,17 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16*) {
 // A value that is the same in all lanes, as one that the compiler knows to be: operands of products and copies then stay in uniform registers.
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
-// Two fp32 values at a time (an instruction of half the issue slots).
-__device__ __forceinline__ void fma2(float& x, float& y, float m, float c) {
-    asm("{\n\t.reg .b64 a, m, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 m, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\tfma.rn.f32x2 a, a, m, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "+f"(x), "+f"(y) : "f"(m), "f"(c));
-}
-__device__ __forceinline__ void add2(float& x, float& y, float u, float v) {
-    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "+f"(x), "+f"(y) : "f"(u), "f"(v));
-}
+// Maxima that are NaN where a value is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-
+__device__ __forceinline__ float max2(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 template <typename T, int HD>
 __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_constant__ PagedParams p) {
     using G = PGeo<HD>;
@@ -327,11 +345,12 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
     }
     const int singles = uniform(single_ctas(p.line, s_cum[p.requests], s_segments, p.kv_heads, ctas));
     const bool pair = cta < ctas - singles;
+    const int ahead = uniform(first_blocks(p.line, ctas - singles));
     if (warp < 2 && lane == 0) {
         // (the streams' workers: first one of every CTA, then the other)
         const Share share = pair ? Share(p.line.pair_total, ctas - singles) : Share(p.line.odd + s_cum[p.requests], 2 * singles);
         const int w = pair ? cta : cta - (ctas - singles) + warp * singles;
-        s_from[warp] = cursor_at(p, s_cum, s_req, pair, share.start(w), share.start(w + 1));
+        s_from[warp] = cursor_at(p, s_cum, s_req, pair, ahead, share.start(w), share.start(w + 1));
     } else if (cta == 0 && warp >= 2) {
         for (int b = threadIdx.x - 64; b <= p.requests; b += kPgThreads - 64) p.plan[b] = s_cum[b];
         if (threadIdx.x == 64) p.plan[p.requests + 1] = singles;
@@ -420,7 +439,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
                 if (s != 0) ask(1, x.c, x.c.tile + (s == 2));
             }
             if (++x.kb == x.kb1) {
-                advance(x.c, p, s_req, s == 2);
+                advance(x.c, p, s_req, s == 2, ahead);
                 x.kb = x.c.kb;
                 x.kb1 = x.c.last();
                 x.ahead = page_at(x, x.kb);
@@ -489,7 +508,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
             __syncwarp();
             x.blocks++;
             if (give) kring++;
-            if (last) advance(x.c, p, s_req, pair);
+            if (last) advance(x.c, p, s_req, pair, ahead);
         };
         // Output of the block whose scores stream s asked for last.
         auto output = [&](int s, const At& x, bool take, bool give) {
@@ -565,7 +584,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
                 limit = min(limit, masked ? old : old + (t - c.r.start) + 1);
                 if (masked && valid) bits = p.mask[t];
             }
-            float m = -INFINITY, sum[2] = {0.f, 0.f};                    // the reference of the row's weights, no more than 2^kLag below its maximum
+            float m = -INFINITY, sum = 0.f;                    // the reference of the row's weights, no more than 2^kLag below its maximum
 #pragma unroll 1
             for (int kb = c.kb; kb < kb1; kb++, blocks++) {
                 mbar_wait_reported(smem_u32(sfull + s), blocks & 1, p.polls, p.err, 31);
@@ -603,34 +622,31 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
                         for (int e = 0; e < 4; e++) x[e] = max3(x[e], a[j + e], a[j + 4 + e]);
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[e] = fmaxf(x[e], a[KEYS - 4 + e]);
-                    float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * p.scale_log2;
+                    for (int e = 0; e < 4; e++) x[e] = max2(x[e], a[KEYS - 4 + e]);
+                    float top = max2(max2(x[0], x[1]), max2(x[2], x[3])) * p.scale_log2;
                     s_part[s][blocks & 1][part][r] = top;
                     row_sync();
-                    top = fmaxf(top, s_part[s][blocks & 1][part ^ 1][r]);
-                    const bool grown = top > m + kLag;                   // (of no key so far: m is minus infinity)
-                    const float al = !grown ? 1.f : (m == -INFINITY ? 0.f : exp2_approx(m - top));
+                    top = max2(top, s_part[s][blocks & 1][part ^ 1][r]);
+                    const bool grown = !(top <= m + kLag);               // (of no key so far: m is minus infinity; NaN stays)
+                    const float al = !grown || m != m ? 1.f : (m == -INFINITY ? 0.f : exp2_approx(m - top));
                     if (grown) m = top;
                     const float ref = m == -INFINITY ? 0.f : -m;
                     const bool rescale = __any_sync(0xffffffffu, grown && valid) && kb > c.kb;      // (the same in the rows' other warp)
                     float more[4] = {0.f, 0.f, 0.f, 0.f};
-                    // The weights go to the beginning of the part's scores, which have been read.
 #pragma unroll
                     for (int h = 0; h < KEYS; h += 32) {
                         uint32_t pk[16];
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
-                            float e0 = a[h + j], e1 = a[h + j + 1];
-                            fma2(e0, e1, p.scale_log2, ref);
-                            e0 = exp2_approx(e0);
-                            e1 = exp2_approx(e1);
-                            add2(more[j & 2], more[(j & 2) + 1], e0, e1);
+                            const float e0 = exp2_approx(fmaf(a[h + j], p.scale_log2, ref)), e1 = exp2_approx(fmaf(a[h + j + 1], p.scale_log2, ref));
+                            more[j & 2] += e0;
+                            more[(j & 2) + 1] += e1;
                             pk[j / 2] = pack2(e0, e1, (T*)nullptr);
                         }
                         tmem_st16(tS + h / 2, pk);
                     }
-                    sum[0] = sum[0] * al + (more[0] + more[2]);
-                    sum[1] = sum[1] * al + (more[1] + more[3]);
+                    const float m0 = more[0] + more[1], m1 = more[2] + more[3];
+                    sum = sum * al + (m0 + m1);
                     if (rescale) {
                         // (the block before has been added: its product was waited for ahead of these scores)
 #pragma unroll
@@ -654,22 +670,22 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
             __syncwarp();
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             if (busy) {
-                float l = sum[0] + sum[1];
+                float l = sum;
                 s_part[s][blocks & 1][part][r] = l;                      // (not where the last block's maximum was)
                 row_sync();
                 l += s_part[s][blocks & 1][part ^ 1][r];
                 const long long row = (long long)t * p.heads + c.hk * p.group + g, all = (long long)p.tokens * p.heads;
                 float* dst;
                 long long at;
-                if (c.kb == 0) {
-                    dst = (c.req < 0 ? p.first_prefix : p.first_own) + row * HD;
-                    at = (c.req < 0 ? 0 : all) + row;
+                if (c.kb == c.head) {
+                    dst = (c.head > 0 ? p.first_behind : (c.req < 0 ? p.first_prefix : p.first_own)) + row * HD;
+                    at = (c.head > 0 ? 2 * all : (c.req < 0 ? 0 : all)) + row;
                 } else {
                     // (pairs: 256 rows a CTA; single streams: 128 a stream, behind them)
                     const int w = cta - (ctas - singles) + s * singles;          // (of single streams)
                     const long long slot = pair ? (long long)cta * 2 * kRows + s * kRows + r : (long long)w * kRows + r;
                     dst = (pair ? p.more_pair : p.more) + slot * HD;
-                    at = 2 * all + (pair ? 0 : (long long)ctas * 2 * kRows) + slot;
+                    at = 3 * all + (pair ? 0 : (long long)ctas * 2 * kRows) + slot;
                 }
                 if (valid && part == 0) p.ml[at] = make_float2(l == l ? m : INFINITY, l);      // (scores of NaN alone leave no maximum, but the row is NaN)
                 const unsigned long long mine = reinterpret_cast<unsigned long long>(dst + part * DIMS);      // (used where the row is valid)
@@ -718,7 +734,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
 #pragma unroll 1
         while (c.w < c.end) {
             run(c);
-            advance(c, p, s_req, pair);
+            advance(c, p, s_req, pair, ahead);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
@@ -753,30 +769,35 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     const Share single(l.odd + p.plan[p.requests], 2 * singles);
     const int hk = head / p.group, g = head - hk * p.group, hs = g / p.tile_heads, in = g - hs * p.tile_heads;
     const long long row = (long long)t * p.heads + head, all = (long long)p.tokens * p.heads;
-    // The row's two segments: their first pieces by row, the others by worker (`more`: of which array, rows of a worker, row in them).
+    // The row's segments, of the prefix, its own, of the prefix again: their first pieces by row, the others by worker (`more`: of which array, rows of a worker, row in them).
     struct Segment {
         int from, to;                            // pieces: the first, then workers from + 1 .. to
         const float *first, *more;
         long long first_ml, more_ml;
         int rows, r;
-    } seg[2];
+    } seg[3];
     {
         const int ts = t / p.tile_tokens, tile = ts * p.head_sets + hs, r = (t - ts * p.tile_tokens) * p.tile_heads + in;
         const bool pair = tile < 2 * l.pairs;
-        Segment& x = seg[0];
         const Share share = pair ? Share(l.pair_total, ctas - singles) : single;
-        const int start = pair ? (hk * l.pairs + tile / 2) * l.nbp : hk * l.nbp;
-        x.from = x.to = -1;
-        if (l.nbp > 0) {
-            x.from = share.owner(start);
-            x.to = share.owner(start + l.nbp - 1);
+        const int ahead = pair ? first_blocks(l, ctas - singles) : l.nbp;
+#pragma unroll
+        for (int part = 0; part < 2; part++) {
+            Segment& x = seg[2 * part];
+            const int blocks = part ? l.nbp - ahead : ahead;
+            const int start = pair ? hk * l.pairs * l.nbp + part * l.pairs * ahead + tile / 2 * blocks : hk * l.nbp;
+            x.from = x.to = -1;
+            if (blocks > 0) {
+                x.from = share.owner(start);
+                x.to = share.owner(start + blocks - 1);
+            }
+            x.first = part ? p.first_behind : p.first_prefix;
+            x.first_ml = part ? 2 * all : 0;
+            x.more = pair ? p.more_pair : p.more;
+            x.more_ml = 3 * all + (pair ? 0 : (long long)ctas * 2 * kRows);
+            x.rows = pair ? 2 * kRows : kRows;
+            x.r = pair ? (tile & 1) * kRows + r : r;
         }
-        x.first = p.first_prefix;
-        x.first_ml = 0;
-        x.more = pair ? p.more_pair : p.more;
-        x.more_ml = 2 * all + (pair ? 0 : (long long)ctas * 2 * kRows);
-        x.rows = pair ? 2 * kRows : kRows;
-        x.r = pair ? (tile & 1) * kRows + r : r;
     }
     {
         const int dt = t - q.start, ts = dt / p.tile_tokens, tile = ts * p.head_sets + hs, r = (dt - ts * p.tile_tokens) * p.tile_heads + in;
@@ -791,11 +812,12 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
         x.first = p.first_own;
         x.first_ml = all;
         x.more = p.more;
-        x.more_ml = 2 * all + (long long)ctas * 2 * kRows;
+        x.more_ml = 3 * all + (long long)ctas * 2 * kRows;
         x.rows = kRows;
         x.r = r;
     }
-    const int n0 = seg[0].from < 0 ? 0 : seg[0].to - seg[0].from + 1, n = n0 + (seg[1].from < 0 ? 0 : seg[1].to - seg[1].from + 1);
+    auto count = [](const Segment& s) { return s.from < 0 ? 0 : s.to - s.from + 1; };
+    const int n0 = count(seg[0]), n1 = n0 + count(seg[1]), n = n1 + count(seg[2]);
     float m = -INFINITY, sum = 0.f, o[N] = {};
 #pragma unroll 1
     for (int base = 0; base < n; base += 32 * WAYS) {
@@ -804,15 +826,15 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
         const float* src = nullptr;
         float2 x = make_float2(-INFINITY, 0.f);
         if (k < n) {
-            const Segment& s = k < n0 ? seg[0] : seg[1];
-            const int j = k < n0 ? k : k - n0, w = s.from + j;
+            auto pick = [&](auto a, auto b, auto c) { return k < n0 ? a : (k < n1 ? b : c); };      // (by value: the segments stay in registers)
+            const int j = k - pick(0, n0, n1), w = pick(seg[0].from, seg[1].from, seg[2].from) + j;
             if (j == 0) {
-                src = s.first + row * HD;
-                x = p.ml[s.first_ml + row];
+                src = pick(seg[0].first, seg[1].first, seg[2].first) + row * HD;
+                x = p.ml[pick(seg[0].first_ml, seg[1].first_ml, seg[2].first_ml) + row];
             } else {
-                const long long at = (long long)w * s.rows + s.r;
-                src = s.more + at * HD;
-                x = p.ml[s.more_ml + at];
+                const long long at = (long long)w * pick(seg[0].rows, seg[1].rows, seg[2].rows) + pick(seg[0].r, seg[1].r, seg[2].r);
+                src = pick(seg[0].more, seg[1].more, seg[2].more) + at * HD;
+                x = p.ml[pick(seg[0].more_ml, seg[1].more_ml, seg[2].more_ml) + at];
             }
         }
         float top = x.x;
@@ -880,7 +902,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
 }
 
 struct Room {
-    size_t prefix, own, pair, more, ml, plan, total;                     // byte offsets
+    size_t prefix, own, behind, pair, more, ml, plan, total;             // byte offsets
     int ctas;
 };
 Room room_of(const b200_paged* c, int ctas) {
@@ -888,10 +910,11 @@ Room room_of(const b200_paged* c, int ctas) {
     const size_t all = (size_t)c->tokens * c->heads, row = (size_t)c->head_dim * 4, pair = (size_t)ctas * 2 * kRows, more = (size_t)2 * ctas * kRows;
     r.ctas = ctas;
     r.own = all * row;
-    r.pair = r.own + all * row;
+    r.behind = r.own + all * row;
+    r.pair = r.behind + all * row;
     r.more = r.pair + pair * row;
     r.ml = r.more + more * row;
-    r.plan = r.ml + (2 * all + pair + more) * sizeof(float2);
+    r.plan = r.ml + (3 * all + pair + more) * sizeof(float2);
     r.total = r.plan + (c->requests + 2) * sizeof(int);
     r.total = (r.total + 15) / 16 * 16;
     return r;
@@ -981,6 +1004,7 @@ int b200_paged_attention(const b200_paged* c, const void* q, long long q_token, 
     const Room r = room_of(c, 148);
     char* ws = static_cast<char*>(workspace);
     p.first_prefix = reinterpret_cast<float*>(ws + r.prefix); p.first_own = reinterpret_cast<float*>(ws + r.own);
+    p.first_behind = reinterpret_cast<float*>(ws + r.behind);
     p.more_pair = reinterpret_cast<float*>(ws + r.pair); p.more = reinterpret_cast<float*>(ws + r.more);
     p.ml = reinterpret_cast<float2*>(ws + r.ml); p.plan = reinterpret_cast<int*>(ws + r.plan);
     p.table = c->page_table; p.lengths = c->lengths; p.row_starts = c->row_starts; p.prefix_pages = prefix_pages; p.mask = mask; p.out = out;

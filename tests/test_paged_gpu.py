@@ -143,6 +143,13 @@ def test_attention_is_the_definition(be, cuda, shape, batch):
     Batch(cuda, *shape, 128, *batch, dtype=HALF if dtype == BF else BF, order="nhd", seed=1).check(be)
 
 
+@pytest.mark.parametrize("hd,prefix,new", [(64, 700, [350, 350]), (128, 1500, [700]), (128, 330, [256, 1, 400, 0, 31]), (64, 2900, [1100])])
+def test_many_tiles_share_a_prefix(be, cuda, hd, prefix, new):
+    """So many tiles of queries that a worker's stretch of a prefix is more than half of it, or all, or several."""
+    Batch(cuda, 32, 8, hd, 64, prefix, [5] * len(new), new, dtype=BF if hd == 64 else HALF).check(be)
+    Batch(cuda, 12, 2, hd, 16, prefix, [200] * len(new), new, seed=2).check(be)
+
+
 @pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 256, 384])
 @pytest.mark.parametrize("order", ["hnd", "nhd"])
 @pytest.mark.parametrize("hd", [64, 128])
