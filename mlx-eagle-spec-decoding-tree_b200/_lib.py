@@ -269,7 +269,7 @@ def require_tensor(what: str, t, dtypes, shape, like: torch.Tensor = None, packe
 
 
 def require_writable(what: str, t: torch.Tensor) -> None:
-    """No two elements of a result share their place by a stride of 0."""
+    """No two elements share their place by a stride of 0."""
     if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
         raise B200Error(f"{what} must not be expanded: its elements share their places")
 

@@ -81,6 +81,9 @@ struct PagedParams {
     void* out;
     float *first_prefix, *first_own, *first_behind, *more_pair, *more;      // pieces [..][HD]
     float2* ml;                                  // (m, l) in the order of the pieces
+    const void *q, *k_pages, *v_pages;           // as memory, for what comes seldom
+    long long q_token, q_head, page_stride, head_stride, row_stride;
+    int pages;
     int* plan;                                   // sums of the own blocks, by request; CTAs for single streams
     long long table_stride, out_token, out_head;
     int requests, tokens, heads, kv_heads, group, tile_heads, tile_tokens, half_tokens, head_sets;
@@ -88,7 +91,6 @@ struct PagedParams {
     int box_rows, table_width, prefix;
     Line line;
     float scale_log2;                            // positive
-    bool negative;                               // ... of a negative scale
     int* err;
     int polls;
 };
@@ -551,15 +553,12 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
             at[s].left = s ? n1 : n0;
             at[s].kb = at[s].kb1 = 0;
         }
-#pragma unroll
-        for (int s = 0; s < 2; s++)
-            if (at[s].left > 0) scores(s, at[s], !pair || s == 0, !pair || s == 1);
 #pragma unroll 1
-        for (int i = 0; i < max(n0, n1); i++)
+        for (int i = -1; i < max(n0, n1); i++)
 #pragma unroll
             for (int s = 0; s < 2; s++) {
                 if (i >= (s ? n1 : n0)) continue;
-                output(s, at[s], !pair || s == 0, !pair || s == 1);
+                if (i >= 0) output(s, at[s], !pair || s == 0, !pair || s == 1);
                 if (at[s].left > 0) scores(s, at[s], !pair || s == 0, !pair || s == 1);
             }
     } else {
@@ -600,10 +599,6 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
                         asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
                         for (int j = 0; j < KEYS; j++) a[j] = __uint_as_float(raw[j]);
-                    }
-                    if (p.negative) {
-#pragma unroll
-                        for (int j = 0; j < KEYS; j++) a[j] = -a[j];
                     }
                     if (key0 + KEYS > sure) {                            // what the row does not see is minus infinity
                         const int o = key0 - old, there = length - key0, n = limit - key0;      // the first key among the new rows; keys there are; keys seen
@@ -818,87 +813,124 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     }
     auto count = [](const Segment& s) { return s.from < 0 ? 0 : s.to - s.from + 1; };
     const int n0 = count(seg[0]), n1 = n0 + count(seg[1]), n = n1 + count(seg[2]);
-    float m = -INFINITY, sum = 0.f, o[N] = {};
+    // (`again`: without the row's own segment, see below)
+    for (bool again = false;; again = true) {
+        float m = -INFINITY, sum = 0.f, o[N] = {};
 #pragma unroll 1
-    for (int base = 0; base < n; base += 32 * WAYS) {
-        // a piece a lane
-        const int k = base + lane * WAYS + way;
-        const float* src = nullptr;
-        float2 x = make_float2(-INFINITY, 0.f);
-        if (k < n) {
-            auto pick = [&](auto a, auto b, auto c) { return k < n0 ? a : (k < n1 ? b : c); };      // (by value: the segments stay in registers)
-            const int j = k - pick(0, n0, n1), w = pick(seg[0].from, seg[1].from, seg[2].from) + j;
-            if (j == 0) {
-                src = pick(seg[0].first, seg[1].first, seg[2].first) + row * HD;
-                x = p.ml[pick(seg[0].first_ml, seg[1].first_ml, seg[2].first_ml) + row];
-            } else {
-                const long long at = (long long)w * pick(seg[0].rows, seg[1].rows, seg[2].rows) + pick(seg[0].r, seg[1].r, seg[2].r);
-                src = pick(seg[0].more, seg[1].more, seg[2].more) + at * HD;
-                x = p.ml[pick(seg[0].more_ml, seg[1].more_ml, seg[2].more_ml) + at];
+        for (int base = 0; base < n; base += 32 * WAYS) {
+            // a piece a lane
+            const int k = base + lane * WAYS + way;
+            const float* src = nullptr;
+            float2 x = make_float2(-INFINITY, 0.f);
+            if (k < n && !(again && k >= n0 && k < n1)) {
+                auto pick = [&](auto a, auto b, auto c) { return k < n0 ? a : (k < n1 ? b : c); };      // (by value: the segments stay in registers)
+                const int j = k - pick(0, n0, n1), w = pick(seg[0].from, seg[1].from, seg[2].from) + j;
+                if (j == 0) {
+                    src = pick(seg[0].first, seg[1].first, seg[2].first) + row * HD;
+                    x = p.ml[pick(seg[0].first_ml, seg[1].first_ml, seg[2].first_ml) + row];
+                } else {
+                    const long long at = (long long)w * pick(seg[0].rows, seg[1].rows, seg[2].rows) + pick(seg[0].r, seg[1].r, seg[2].r);
+                    src = pick(seg[0].more, seg[1].more, seg[2].more) + at * HD;
+                    x = p.ml[pick(seg[0].more_ml, seg[1].more_ml, seg[2].more_ml) + at];
+                }
+            }
+            float top = x.x;
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            if (top == -INFINITY) continue;                                  // (the same in all lanes)
+            const float high = fmaxf(m, top), before = exp2_approx(m - high), weight = x.x == -INFINITY ? 0.f : exp2_approx(x.x - high);
+            float l2 = weight * x.y;
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) l2 += __shfl_xor_sync(0xffffffffu, l2, d);
+            sum = sum * before + l2;
+            m = high;
+#pragma unroll
+            for (int e = 0; e < N; e++) o[e] *= before;
+            unsigned left = __ballot_sync(0xffffffffu, weight > 0.f || weight != weight);      // (NaN: scores of NaN make the row NaN)
+            while (left) {
+                float w[BATCH];
+                Vec<float, N> v[BATCH];
+#pragma unroll
+                for (int b = 0; b < BATCH; b++) {                            // (loads of several pieces in flight)
+                    const int j = left ? __ffs(left) - 1 : 0;
+                    const float* from = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), j));
+                    w[b] = __shfl_sync(0xffffffffu, weight, j);
+                    if (left) load_vec<true>(v[b], from + lane * N, N);
+                    else w[b] = 0.f;
+                    if (w[b] == 0.f)
+#pragma unroll
+                        for (int e = 0; e < N; e++) v[b].v[e] = 0.f;
+                    left &= left - 1;
+                }
+#pragma unroll
+                for (int b = 0; b < BATCH; b++)
+#pragma unroll
+                    for (int e = 0; e < N; e++) o[e] += w[b] * v[b].v[e];
             }
         }
-        float top = x.x;
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        if (top == -INFINITY) continue;                                  // (the same in all lanes)
-        const float high = fmaxf(m, top), before = exp2_approx(m - high), weight = x.x == -INFINITY ? 0.f : exp2_approx(x.x - high);
-        float l2 = weight * x.y;
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) l2 += __shfl_xor_sync(0xffffffffu, l2, d);
-        sum = sum * before + l2;
-        m = high;
-#pragma unroll
-        for (int e = 0; e < N; e++) o[e] *= before;
-        unsigned left = __ballot_sync(0xffffffffu, weight > 0.f || weight != weight);      // (NaN: scores of NaN make the row NaN)
-        while (left) {
-            float w[BATCH];
-            Vec<float, N> v[BATCH];
-#pragma unroll
-            for (int b = 0; b < BATCH; b++) {                            // (loads of several pieces in flight)
-                const int j = left ? __ffs(left) - 1 : 0;
-                const float* from = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), j));
-                w[b] = __shfl_sync(0xffffffffu, weight, j);
-                if (left) load_vec<true>(v[b], from + lane * N, N);
-                else w[b] = 0.f;
-                if (w[b] == 0.f)
-#pragma unroll
-                    for (int e = 0; e < N; e++) v[b].v[e] = 0.f;
-                left &= left - 1;
+        if constexpr (WAYS > 1) {
+            __shared__ float s_m[WAYS], s_sum[WAYS], s_o[WAYS][HD];
+            if (again) __syncthreads();
+            if (lane == 0) {
+                s_m[way] = m;
+                s_sum[way] = sum;
             }
 #pragma unroll
-            for (int b = 0; b < BATCH; b++)
+            for (int e = 0; e < N; e++) s_o[way][lane * N + e] = o[e];
+            __syncthreads();
+            m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+            sum = 0.f;
 #pragma unroll
-                for (int e = 0; e < N; e++) o[e] += w[b] * v[b].v[e];
-        }
-    }
-    if constexpr (WAYS > 1) {
-        __shared__ float s_m[WAYS], s_sum[WAYS], s_o[WAYS][HD];
-        if (lane == 0) {
-            s_m[way] = m;
-            s_sum[way] = sum;
-        }
+            for (int e = 0; e < N; e++) o[e] = 0.f;
 #pragma unroll
-        for (int e = 0; e < N; e++) s_o[way][lane * N + e] = o[e];
-        __syncthreads();
+            for (int w = 0; w < WAYS; w++) {                                 // (in order: the same bits every time)
+                if (s_m[w] == -INFINITY) continue;
+                const float a = exp2_approx(s_m[w] - m);
+                sum += a * s_sum[w];
+#pragma unroll
+                for (int e = 0; e < N; e++) o[e] += a * s_o[w][lane * N + e];
+            }
+        }
+        if (!again) {
+            // Inf and NaN in the values of new rows that this row does not see have come in as 0 x Inf or NaN.  That is seldom: where anything is not finite, the
+            // row's own rows are gone through one by one, and those that it does not see are left out.
+            bool bad = !(fabsf(sum) < INFINITY);
+#pragma unroll
+            for (int e = 0; e < N; e++) bad = bad || !(fabsf(o[e]) < INFINITY);
+            if (__any_sync(0xffffffffu, bad)) continue;                      // (of four warps, all)
+        } else {
+            const T* mine = static_cast<const T*>(p.q) + t * p.q_token + head * p.q_head + lane * N;
+            float x[N];
+#pragma unroll
+            for (int e = 0; e < N; e++) x[e] = to_f32(mine[e]) * p.scale_log2;
+#pragma unroll 1
+            for (int key = 0; key < q.length; key++) {
+                const int j = key - q.old;                                   // which new row
+                if (p.mask != nullptr ? j >= 0 && (j > 63 || !((p.mask[t] >> j) & 1)) : j > t - q.start) continue;
+                const int page = p.table[lo * p.table_stride + key / p.page_size];
+                const bool there = page >= 0 && page < p.pages;
+                const long long at = page * p.page_stride + hk * p.head_stride + key % p.page_size * p.row_stride + lane * N;
+                float s = 0.f;
+                if (there)
+#pragma unroll
+                    for (int e = 0; e < N; e++) s += x[e] * to_f32(static_cast<const T*>(p.k_pages)[at + e]);
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+                const float high = s == s ? fmaxf(m, s) : s, a = m == high ? 1.f : exp2_approx(m - high), w = exp2_approx(s - high);
+                sum = sum * a + w;
+#pragma unroll
+                for (int e = 0; e < N; e++) o[e] = o[e] * a + (there ? w * to_f32(static_cast<const T*>(p.v_pages)[at + e]) : 0.f);
+                m = high;
+            }
+        }
         if (way > 0) return;
-        m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-        sum = 0.f;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        Vec<T, N> y;
 #pragma unroll
-        for (int e = 0; e < N; e++) o[e] = 0.f;
-#pragma unroll
-        for (int w = 0; w < WAYS; w++) {                                 // (in order: the same bits every time)
-            if (s_m[w] == -INFINITY) continue;
-            const float a = exp2_approx(s_m[w] - m);
-            sum += a * s_sum[w];
-#pragma unroll
-            for (int e = 0; e < N; e++) o[e] += a * s_o[w][lane * N + e];
-        }
+        for (int e = 0; e < N; e++) y.v[e] = from_f32<T>(o[e] * inv);
+        store_vec<true>(static_cast<T*>(p.out) + t * p.out_token + head * p.out_head + lane * N, y, N);
+        return;
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    Vec<T, N> y;
-#pragma unroll
-    for (int e = 0; e < N; e++) y.v[e] = from_f32<T>(o[e] * inv);
-    store_vec<true>(static_cast<T*>(p.out) + t * p.out_token + head * p.out_head + lane * N, y, N);
 }
 
 struct Room {
@@ -960,7 +992,7 @@ int b200_paged_attention(const b200_paged* c, const void* q, long long q_token, 
     using namespace b200;
     const int bad = check_paged(c);
     if (bad != B200_OK) return bad;
-    if ((c->head_dim != 64 && c->head_dim != 128) || prefix_length < 0 || (prefix_length > 0 && !prefix_pages)) return B200_EINVAL;
+    if ((c->head_dim != 64 && c->head_dim != 128) || !(scale >= 0.f) || prefix_length < 0 || (prefix_length > 0 && !prefix_pages)) return B200_EINVAL;
     if ((c->page_size < 128 && (c->page_size < 8 || (c->page_size & (c->page_size - 1)))) || (c->page_size > 128 && c->page_size % 128)) return B200_EINVAL;
     if (c->requests > kPgMaxRequests) return B200_ELIMIT;
     if (c->tokens == 0 || c->requests == 0) return B200_OK;
@@ -968,6 +1000,11 @@ int b200_paged_attention(const b200_paged* c, const void* q, long long q_token, 
     if (workspace_bytes < b200_paged_attention_workspace_bytes(c)) return B200_EWORKSPACE;
     if (!aligned16(q) || !aligned16(out) || !aligned16(c->k_pages) || !aligned16(c->v_pages) || !aligned16(workspace)) return B200_EALIGN;
     if (q_token % 8 || q_head % 8 || out_token % 8 || out_head % 8 || c->page_stride % 8 || c->head_stride % 8 || c->row_stride % 8) return B200_EALIGN;
+
+    // (a tensor map has no strides of 0)
+    if ((c->tokens > 1 && q_token <= 0) || (c->heads > 1 && q_head <= 0) || (c->page_size > 1 && c->row_stride <= 0) || (c->kv_heads > 1 && c->head_stride <= 0) ||
+        (c->pages > 1 && c->page_stride <= 0))
+        return B200_EINVAL;
 
     PagedParams p{};
     p.group = c->heads / c->kv_heads;
@@ -1008,6 +1045,8 @@ int b200_paged_attention(const b200_paged* c, const void* q, long long q_token, 
     p.more_pair = reinterpret_cast<float*>(ws + r.pair); p.more = reinterpret_cast<float*>(ws + r.more);
     p.ml = reinterpret_cast<float2*>(ws + r.ml); p.plan = reinterpret_cast<int*>(ws + r.plan);
     p.table = c->page_table; p.lengths = c->lengths; p.row_starts = c->row_starts; p.prefix_pages = prefix_pages; p.mask = mask; p.out = out;
+    p.q = q; p.k_pages = c->k_pages; p.v_pages = c->v_pages; p.q_token = q_token; p.q_head = q_head;
+    p.page_stride = c->page_stride; p.head_stride = c->head_stride; p.row_stride = c->row_stride; p.pages = c->pages;
     p.table_stride = c->table_stride; p.out_token = out_token; p.out_head = out_head;
     p.requests = c->requests; p.tokens = c->tokens; p.heads = c->heads; p.kv_heads = c->kv_heads;
     p.page_size = c->page_size; p.page_blocks = c->page_size / kKeys; p.box_rows = box;
@@ -1019,8 +1058,7 @@ int b200_paged_attention(const b200_paged* c, const void* q, long long q_token, 
     p.line.pair_total = c->kv_heads * p.line.pairs * p.line.nbp;
     p.table_width = c->table_width; p.prefix = prefix_length;
     // (of a scale of nothing, weights are equal; a positive one, however small, keeps hidden scores at minus infinity)
-    p.negative = scale < 0.f;
-    p.scale_log2 = std::max(std::abs(scale) * 1.4426950408889634f, 1e-30f);
+    p.scale_log2 = std::max(scale * 1.4426950408889634f, 1e-30f);
     p.err = error;
     p.polls = wait_polls(kWaitPolls, kFirmPolls / 2);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -129,6 +129,8 @@ def _error_word(device) -> torch.Tensor:
     """One word per device that a wait inside the attention sets when it runs out; never freed, captured passes hold its address."""
     word = _errors.get(device.index)
     if word is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise _lib.B200Error("the first attention on a device must not be captured: its error word would belong to the graph")
         word = _errors[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
     return word
 
@@ -141,7 +143,8 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     older rows are seen by all; new rows from the 64th on are hidden).
 
     ``q (tokens, heads, dim)``, positions already in it; heads of 64 or 128; float16 or bfloat16, scores, statistics and sums in fp32, probabilities
-    rounded to the type for the second product.  ``scale`` is ``dim ** -0.5`` unless given.  A token that sees no row gets zeros.  Rows behind a
+    rounded to the type for the second product; NaN and infinities reach the tokens that see them, and no other.  ``out`` may be ``q``.  ``scale``, 0 or more, is
+    ``dim ** -0.5`` unless given.  A token that sees no row gets zeros.  Rows behind a
     length may hold anything; a page number outside the cache stands for rows of zeros.  At most 1024 requests."""
     if out is None and isinstance(q, torch.Tensor):
         y = _lib.ops().paged_attention(q, k_pages, v_pages, page_table, lengths, row_starts, prefix_pages, prefix_length, mask, scale,
@@ -159,6 +162,9 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
         _lib.require_tensor("prefix_pages", prefix_pages, (torch.int32,), (None,), q)
         if prefix_pages.numel() * c.page_size < prefix_length:
             raise _lib.B200Error(f"{prefix_pages.numel()} pages of {c.page_size} rows cannot hold a prefix of {prefix_length}")
+    scale = c.head_dim ** -0.5 if scale is None else float(scale)
+    if not scale >= 0.0:
+        raise _lib.B200Error(f"attention takes a scale of 0 or more, not {scale}")
     if mask is not None:
         _lib.require_tensor("mask", mask, (torch.int64,), (c.tokens,), q)
     if out is None:
@@ -166,13 +172,14 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     else:
         _lib.require_tensor("out", out, (q.dtype,), q.shape, q, packed=False)
         _lib.require_writable("out", out)
+    _lib.require_writable("q", q)
     if any(s % 8 for t in (q, out, k_pages) for s in t.stride()[:-1]) or any(t.data_ptr() % 16 for t in (q, out, k_pages, v_pages)):
         raise _lib.B200Error("attention needs rows that start at 16 bytes: q, out and pages with strides of multiples of 8")
     L = _lib.lib()
     with _lib.on_device(q):
         ws = torch.empty(L.b200_paged_attention_workspace_bytes(ctypes.byref(c)), dtype=torch.uint8, device=q.device)
         rc = L.b200_paged_attention(ctypes.byref(c), _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(out), out.stride(0), out.stride(1),
-                                    _lib.ptr(prefix_pages), int(prefix_length), _lib.ptr(mask), c.head_dim ** -0.5 if scale is None else float(scale),
+                                    _lib.ptr(prefix_pages), int(prefix_length), _lib.ptr(mask), scale,
                                     _lib.ptr(ws), ws.numel(), _lib.ptr(_error_word(q.device)), _lib.stream_ptr(q.device))
     _lib.check(rc, "b200_paged_attention")
     return out

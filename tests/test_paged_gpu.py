@@ -167,8 +167,8 @@ def test_masks_of_drafted_trees(be, cuda, shape, prefix, old, new, dtype):
         assert (got[0] == 0).all()                                       # a token that sees nothing
 
 
-@pytest.mark.parametrize("spread,scale", [(30.0, None), (2.0, 1.0), (2.0, 0.0), (2.0, -0.1)])
-def test_peaked_flat_and_negative_scales(be, cuda, spread, scale):
+@pytest.mark.parametrize("spread,scale", [(30.0, None), (2.0, 1.0), (2.0, 0.0)])
+def test_peaked_and_flat_scales(be, cuda, spread, scale):
     for dtype in (HALF, BF):
         Batch(cuda, 8, 2, 128, 16, 600, [50, 600], [3, 2], dtype=dtype, spread=spread).check(be, scale=scale)
 
@@ -184,6 +184,37 @@ def test_growing_scores_leave_earlier_maxima_far_behind(be, cuda):
         b._put(b.table[i].tolist(), r)
     b.q = b.q.abs()
     b.check(be)
+
+
+@pytest.mark.parametrize("dtype", [HALF, BF], ids=str)
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("hd,prefix,old,new", [(64, 0, [0, 3], [9, 1]), (128, 300, [125, 700, 1], [7, 1, 40]), (128, 0, [60], [130])])
+def test_nan_and_infinities_reach_those_who_see_them(be, cuda, hd, prefix, old, new, tree, dtype):
+    """New rows whose values or keys are not finite: a token that does not see them (a later row, another branch of the tree) gets what it
+    gets without them, within the tolerance; one that does is not finite in those dims, or, for a key, NaN in all."""
+    def batch():
+        b = Batch(cuda, 8, 2, hd, 16, prefix, old, new, dtype=dtype)
+        return b.tree(empty=True) if tree else b
+    b = batch()
+    want = b.run(be)
+    exact, tol = b.exact()
+    at, hit = 0, torch.zeros(sum(new), 8, hd, dtype=torch.bool, device=cuda)
+    for r, n in enumerate(new):
+        for j, head, what, key in ((n - 1, 0, math.inf, False), (n // 2, 1, math.nan, False), (n // 3, 0, -math.inf, False), (n - 2, 1, math.nan, True)):
+            if j < 0:
+                continue
+            dims = slice(0, hd) if key else slice(3 * j % hd, 3 * j % hd + 1)
+            b.rows[r][0 if key else 1, head, old[r] + j, 7 if key else dims] = what
+            for i in range(n):
+                sees = j <= i if not tree else j < 64 and bool((int(b.mask[at + i]) >> j) & 1)
+                if sees:
+                    hit[at + i, 4 * head: 4 * head + 4, dims] = True
+        at += n
+        b._put(b.table[r].tolist(), b.rows[r])
+    got = b.run(be)
+    assert not got[hit].isfinite().any() and ((got.double() - exact).abs() <= tol)[~hit].all()
+    b = batch()                                                          # and nothing of it is left for the next call
+    assert torch.equal(b.run(be), want) and be.paged.attention_error(cuda) == 0
 
 
 def test_a_prefix_counts_like_rows_of_its_own(be, cuda):
@@ -348,9 +379,9 @@ def test_paged_refusals(be, cuda):
              lambda: at(*changed(1, b.k_pages[:, :1])), lambda: at(*changed(2, b.v_pages.transpose(1, 2).contiguous().transpose(1, 2))),
              lambda: at(*changed(3, b.table.long())), lambda: at(*changed(3, b.table[:1])), lambda: at(*changed(4, b.lengths.long())),
              lambda: at(*changed(5, b.row_starts[:2])), lambda: at(*base, prefix_length=5), lambda: at(*base, prefix_pages=b.prefix_pages, prefix_length=33),
-             lambda: at(*base, prefix_length=-1), lambda: at(*base, mask=torch.zeros(5, dtype=torch.int64, device=cuda)),
+             lambda: at(*base, prefix_length=-1), lambda: at(*base, scale=-0.1), lambda: at(*base, scale=math.nan), lambda: at(*base, mask=torch.zeros(5, dtype=torch.int64, device=cuda)),
              lambda: at(*base, mask=torch.zeros(6, dtype=torch.int32, device=cuda)), lambda: at(*base, out=b.q[:5]), lambda: at(*base, out=b.q.float()),
-             lambda: at(*changed(0, torch.zeros(6, 4, 68, device=cuda).half()[..., 1:65])),
+             lambda: at(*changed(0, b.q[:1].expand(6, 4, 64))), lambda: at(*changed(0, torch.zeros(6, 4, 68, device=cuda).half()[..., 1:65])),
              lambda: at(b.q[..., :32], b.k_pages[..., :32], b.v_pages[..., :32], *base[3:]),
              lambda: at(b.q, b.k_pages[:, :, :12], b.v_pages[:, :, :12], *base[3:]),
              lambda: ap(b.q, k[:5], k, *base[1:], inv), lambda: ap(b.q, k, k[:, :1], *base[1:], inv), lambda: ap(b.q, k, k, *base[1:], inv[:0]),

@@ -57,8 +57,8 @@ def test_append_entry(be):
 def test_attention_entry(be):
     lib, (buf, base) = be._lib.lib(), _memory()
 
-    def call(c, q=base, q_token=256, prefix=None, length=0, ws=base, room=1 << 40, error=base):
-        return lib.b200_paged_attention(ctypes.byref(c), q, q_token, 64, base, 256, 64, prefix, length, None, 0.125, ws, room, error, None)
+    def call(c, q=base, q_token=256, prefix=None, length=0, ws=base, room=1 << 40, error=base, scale=0.125):
+        return lib.b200_paged_attention(ctypes.byref(c), q, q_token, 64, base, 256, 64, prefix, length, None, scale, ws, room, error, None)
 
     assert lib.b200_paged_attention_workspace_bytes(ctypes.byref(_cache(be, base))) > 0
     assert lib.b200_paged_attention_workspace_bytes(ctypes.byref(_cache(be, base, kv_heads=3))) == 0
@@ -67,6 +67,7 @@ def test_attention_entry(be):
     assert call(_cache(be, base, requests=1025)) == -6
     assert call(_cache(be, base), length=5) == call(_cache(be, base), prefix=base, length=-1) == -1
     assert call(_cache(be, base), q=None) == call(_cache(be, base), ws=None) == call(_cache(be, base), error=None) == -1
+    assert call(_cache(be, base), scale=-1.0) == call(_cache(be, base), scale=float("nan")) == -1
     assert call(_cache(be, base), room=0) == -4
     assert call(_cache(be, base), q=base + 2) == call(_cache(be, base), q_token=257) == call(_cache(be, base, row_stride=65)) == -2
     assert call(_cache(be, base, tokens=0)) == 0
