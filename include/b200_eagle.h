@@ -551,8 +551,9 @@ int b200_paged_append(const b200_paged* c, const b200_rotary* r, const void* q, 
 /* out[t][h] = softmax(scale * q . K) V over the rows of the shared prefix (prefix_pages, prefix_length rows; NULL and 0: none) and those of
  * the token's own request: causal, or by `mask`: one word a token, bit j = the token sees the request's j-th new row (rows from the 64th
  * on are hidden); older rows are seen by all.  A token that sees nothing gets zeros; tokens that are nobody's are left alone.  Rows behind the
- * last may hold anything; a page number outside the cache stands for rows of zeros.  head_dim 64 or 128; page_size 8, 16, 32, 64 or a multiple of
- * 128; strides multiples of 8, pointers 16-byte aligned; at most 1024 requests.
+ * last may hold anything, so may rows that a token does not see; a score of NaN among those that it sees makes its output NaN.  A page number
+ * outside the cache stands for rows of zeros.  out may be q with the same strides.  scale is finite and 0 or more.  head_dim 64 or 128; page_size 8,
+ * 16, 32, 64 or a multiple of 128; strides positive multiples of 8, pointers 16-byte aligned; at most 1024 requests.
  * workspace: b200_paged_attention_workspace_bytes(c) bytes, 16-byte aligned, of any content, not shared with a call that may run at the same
  * time.  error: device word, zero at first; not zero after a wait inside the kernel that ran out. */
 size_t b200_paged_attention_workspace_bytes(const b200_paged* c);

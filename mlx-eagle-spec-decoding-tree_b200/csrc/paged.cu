@@ -14,7 +14,7 @@
 // tiles of queries or more, the CTA takes them in pairs, a tile a stream, over the same blocks: keys and values are then copied once for 256
 // rows.  Keys and values come page by page (TMA, boxes of a page or 128 rows) into one ring, blocks of the streams in turn.
 //
-// Probabilities are at most one and rounded to the type of V for the second product; scores, statistics, sums and outputs are fp32.
+// Weights are at most 2^kLag and rounded to the type of V for the second product; scores, statistics, sums and outputs are fp32.
 // Every wait is bounded; one that runs out sets the error word and goes on.  No copy uses cluster multicast.
 #include <algorithm>
 #include <atomic>
@@ -742,7 +742,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
 
 // A warp joins the pieces of one query row: a lane looks at a piece's statistics, then all lanes add its output, four dims (two) each.  With WAYS
 // of 4 a row has the four warps of a CTA, every fourth piece each: where there are few rows, they have many pieces, and too few warps to have
-// their loads in flight.
+// their loads in flight.  (512 rows of 16 requests behind 16384 rows: attention in 29.6 us, by one warp a row 32.9; 2048 rows of 64: 60.4 and
+// 58.0.)
 template <typename T, int HD, int WAYS>
 __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedParams p, int ctas) {
     pdl_launch_dependents();
@@ -899,6 +900,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
             for (int e = 0; e < N; e++) bad = bad || !(fabsf(o[e]) < INFINITY);
             if (__any_sync(0xffffffffu, bad)) continue;                      // (of four warps, all)
         } else {
+            if (way > 0) return;
             const T* mine = static_cast<const T*>(p.q) + t * p.q_token + head * p.q_head + lane * N;
             float x[N];
 #pragma unroll
@@ -916,14 +918,14 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
                     for (int e = 0; e < N; e++) s += x[e] * to_f32(static_cast<const T*>(p.k_pages)[at + e]);
 #pragma unroll
                 for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-                const float high = s == s ? fmaxf(m, s) : s, a = m == high ? 1.f : exp2_approx(m - high), w = exp2_approx(s - high);
+                const float high = s == s ? fmaxf(m, s) : s, a = m == high ? 1.f : exp2_approx(m - high), w = s == -INFINITY ? 0.f : exp2_approx(s - high);
                 sum = sum * a + w;
 #pragma unroll
                 for (int e = 0; e < N; e++) o[e] = o[e] * a + (there ? w * to_f32(static_cast<const T*>(p.v_pages)[at + e]) : 0.f);
                 m = high;
             }
         }
-        if (way > 0) return;
+        if (WAYS > 1 && way > 0) return;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         Vec<T, N> y;
 #pragma unroll
@@ -968,7 +970,7 @@ int launch_paged(const PagedParams& p, int ctas, cudaStream_t stream) {
     const int rc = launch_chain(kern, dim3(ctas), kPgThreads, PGeo<HD>::SMEM, 1, stream, p);
     if (rc != B200_OK) return rc;
     // (a row a CTA as long as its warps find room at once)
-    if ((long long)p.tokens * p.heads <= 16 * ctas) launch_kernel(paged_join_kernel<T, HD, 4>, dim3(p.tokens, p.heads), dim3(128), 0, stream, p, ctas);
+    if ((long long)p.tokens * p.heads <= 8 * ctas) launch_kernel(paged_join_kernel<T, HD, 4>, dim3(p.tokens, p.heads), dim3(128), 0, stream, p, ctas);
     else launch_kernel(paged_join_kernel<T, HD, 1>, dim3(p.tokens, (p.heads + 3) / 4), dim3(128), 0, stream, p, ctas);
     return check_launch();
 }
@@ -992,7 +994,7 @@ int b200_paged_attention(const b200_paged* c, const void* q, long long q_token, 
     using namespace b200;
     const int bad = check_paged(c);
     if (bad != B200_OK) return bad;
-    if ((c->head_dim != 64 && c->head_dim != 128) || !(scale >= 0.f) || prefix_length < 0 || (prefix_length > 0 && !prefix_pages)) return B200_EINVAL;
+    if ((c->head_dim != 64 && c->head_dim != 128) || !(scale >= 0.f && scale <= 3e38f) || prefix_length < 0 || (prefix_length > 0 && !prefix_pages)) return B200_EINVAL;
     if ((c->page_size < 128 && (c->page_size < 8 || (c->page_size & (c->page_size - 1)))) || (c->page_size > 128 && c->page_size % 128)) return B200_EINVAL;
     if (c->requests > kPgMaxRequests) return B200_ELIMIT;
     if (c->tokens == 0 || c->requests == 0) return B200_OK;

@@ -234,8 +234,9 @@ int launch_rotary(RotParams& p, bool interleaved, cudaStream_t stream) {
               p.page_head % VE == 0 && p.page_row % VE == 0;
     const int ve = vec ? VE : 2, heads = APPEND ? p.heads + 2 * p.kv_heads : p.heads;
     const int items = ((interleaved ? rot : p.half) + ve - 1) / ve + (p.dim - rot + ve - 1) / ve, sweep = std::max(kRotThreads / items, 1);
-    // Two tokens a CTA where there are CTAs enough; where there are few, the heads of one go to several.
-    p.per_cta = p.tokens >= 8 * 148 ? kRotTokens : 1;
+    // Two tokens a CTA where there are CTAs enough (4099 tokens 9.2 us, 13.1 by one token a CTA; 600 tokens 3.2 and 3.5); where there are few, the
+    // heads of one go to several (16 tokens appended 3.6 us, 4.1 by two tokens a CTA).
+    p.per_cta = p.tokens >= 4 * 148 ? kRotTokens : 1;
     const int gy = p.tokens >= 2 * 148 ? 1 : std::min((heads + sweep * kRotSweeps - 1) / (sweep * kRotSweeps), 65535);
     const dim3 grid((p.tokens + p.per_cta - 1) / p.per_cta, gy);
     const size_t smem = sizeof(float2) * p.half * p.per_cta;

@@ -163,8 +163,8 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
         if prefix_pages.numel() * c.page_size < prefix_length:
             raise _lib.B200Error(f"{prefix_pages.numel()} pages of {c.page_size} rows cannot hold a prefix of {prefix_length}")
     scale = c.head_dim ** -0.5 if scale is None else float(scale)
-    if not scale >= 0.0:
-        raise _lib.B200Error(f"attention takes a scale of 0 or more, not {scale}")
+    if not 0.0 <= scale <= 3e38:
+        raise _lib.B200Error(f"attention takes a finite scale of 0 or more, not {scale}")
     if mask is not None:
         _lib.require_tensor("mask", mask, (torch.int64,), (c.tokens,), q)
     if out is None:

@@ -393,3 +393,151 @@ def test_paged_refusals(be, cuda):
     empty = torch.zeros(0, 4, 64, device=cuda).half()
     none = dict(page_table=b.table[:0], lengths=b.lengths[:0], row_starts=b.row_starts[:1])
     assert at(empty, b.k_pages, b.v_pages, **none).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("shape", [(8, 2, 128), (14, 2, 64)], ids=str)
+def test_calls_at_once_captured_and_in_place(be, cuda, shape):
+    """Passes side by side on two streams, by calls and by two graphs replayed in turn and at once, have a workspace each: bit for bit what
+    one call after the other gives; so has a result that takes the queries' place."""
+    heads, kv, hd = shape
+    a = Batch(cuda, heads, kv, hd, 16, 5000, [700, 90, 0], [3, 40, 1])
+    b = Batch(cuda, heads, kv, hd, 32, 1000, [300] * 5, [4] * 5, seed=1).tree()
+    want = [x.check(be).clone() for x in (a, b)]
+    here, side = torch.cuda.current_stream(), torch.cuda.Stream()
+    side.wait_stream(here)
+    got = []
+    for _ in range(5):
+        got.append((0, a.run(be)))
+        with torch.cuda.stream(side):
+            got.append((1, b.run(be)))
+    graphs, out = [], []
+    torch.cuda.synchronize()
+    for x in (a, b):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            out.append(x.run(be))
+    for turn in range(4):
+        for o in out:
+            o.zero_()
+        side.wait_stream(here)
+        graphs[0].replay()
+        with torch.cuda.stream(side if turn % 2 else here):
+            graphs[1].replay()
+        here.wait_stream(side)
+        got += [(0, out[0].clone()), (1, out[1].clone())]
+    torch.cuda.synchronize()
+    for i, o in got:
+        assert torch.equal(o, want[i])
+    for x, w in zip((a, b), want):
+        assert x.run(be, out=x.q) is x.q and torch.equal(x.q, w)
+    assert be.paged.attention_error(cuda) == 0
+
+
+def test_the_first_attention_is_not_captured(be, cuda, monkeypatch):
+    b = Batch(cuda, 4, 2, 64, 16, 20, [14, 0], [4, 2])
+    want = b.run(be)
+    monkeypatch.setattr(be.paged, "_errors", {})
+    with pytest.raises(be._lib.B200Error, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            b.run(be)
+    assert torch.equal(b.run(be), want)
+
+
+def test_as_many_requests_as_are_taken(be, cuda):
+    Batch(cuda, 4, 1, 64, 8, 100, [i % 11 for i in range(1024)], [1 + (i % 7 == 0) for i in range(1024)]).check(be)
+    Batch(cuda, 4, 1, 64, 8, 0, [0] * 1024, [i % 2 for i in range(1024)]).check(be)
+    more = Batch(cuda, 4, 1, 64, 8, 0, [0] * 1025, [1] * 1025)
+    with pytest.raises(be._lib.B200Error):
+        more.run(be)
+
+
+def test_scores_of_minus_infinity_weigh_nothing(be, cuda):
+    """A key whose scores are minus infinity, first of a request without a prefix, counts as if it were hidden; also where a value that is not
+    seen makes the row be looked at again."""
+    b = Batch(cuda, 4, 2, 64, 16, 0, [3], [2])
+    b.q[..., 0] = 1.0
+    b.rows[0][0, :, 0, 0] = -math.inf
+    b.rows[0][1, :, 4, 5] = math.inf                                     # (of the last token, which the one before it does not see)
+    b._put(b.table[0].tolist(), b.rows[0])
+    got = b.run(be)
+    q, (k, v) = b.q[0].double(), b.rows[0][:, :, 1:4].double()
+    k, v = k.repeat_interleave(2, 0), v.repeat_interleave(2, 0)
+    p = torch.softmax(torch.einsum("hd,hnd->hn", q, k) / 8, -1)
+    want, size = torch.einsum("hn,hnd->hd", p, v), torch.einsum("hn,hnd->hd", p, v.abs())
+    big = float(torch.einsum("hd,hnd->hn", q.abs(), k.abs()).max()) / 8
+    tol = 2.0 ** -11 * want.abs() + (2 * 2.0 ** -11 + 2 * 2.0 ** -20 * big + 2.0 ** -18) * size + 2.0 ** -25 * (1 + 5 * float(v.abs().max()))
+    assert ((got[0].double() - want).abs() <= tol).all()
+    assert got[1, :, 5].isinf().all() and got[1, :, 6:].isfinite().all()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_speculation_writes_what_plain_steps_write(be, cuda, interleaved):
+    """Requests behind a shared prompt, drafts of mixed quality: append, attention and verification together give the tokens that a model in 64
+    bits without a cache gives, and accept just the drafts that agree.  (The best logit is ahead by more than 0.1 at every place, by the 64-bit model.
+    Here half-step roundings of q, k, probabilities and results move an output by 6e-4, as a standard deviation, and a logit of 384 of them by 0.012.)"""
+    heads, kv, hd, page, V, prompt, B, K, total = 6, 2, 64, 16, 61, 43, 3, 3, 24
+    g = torch.Generator().manual_seed(9)
+    table_of = torch.randn(V, heads + 2 * kv, hd, generator=g).half()
+    W = torch.randn(heads * hd, V, generator=g).half()
+    inv, scaling, mag = be.rope.frequencies(hd, 1e4)
+    text = torch.randint(0, V, (prompt,), generator=g).tolist()
+    starts = torch.randint(0, V, (B,), generator=g).tolist()
+
+    def turn(x):
+        pos = torch.arange(x.shape[0], dtype=torch.float64)[:, None] * inv.double()
+        c, s = pos.cos()[:, None], pos.sin()[:, None]
+        a, b = (x[..., ::2], x[..., 1::2]) if interleaved else (x[..., :hd // 2], x[..., hd // 2:])
+        y = (a * c - b * s, b * c + a * s)
+        return torch.stack(y, -1).flatten(-2) if interleaved else torch.cat(y, -1)
+
+    def after(tokens):
+        x = table_of[tokens].double()
+        q, k = turn(x)[-1, :heads], turn(x)[:, heads:heads + kv].repeat_interleave(heads // kv, 1)
+        p = torch.softmax(torch.einsum("hd,nhd->hn", q, k) / 8, -1)
+        logits = torch.einsum("hn,nhd->hd", p, x[:, heads + kv:].repeat_interleave(heads // kv, 1)).flatten() @ W.double()
+        best = logits.topk(2).values
+        assert best[0] - best[1] > 0.1
+        return int(logits.argmax())
+
+    want = []
+    for b in range(B):
+        mine = [starts[b]]
+        for _ in range(total + K + 1):
+            mine.append(after(text + mine))
+        want.append(mine)
+
+    cache = be.PagedKVCache(1, 32, page, kv, hd, device=cuda)
+    k_pages, v_pages = cache.layer(0)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)
+    prefix = ints(cache.take(prompt))
+    table = ints([cache.take(total + 2 * K + 2) for _ in range(B)])
+    E, proj = table_of.to(cuda), W.float().to(cuda)
+    inv = inv.to(cuda)
+
+    def put(tokens, pages, lengths, row_starts, ahead):
+        x = E[tokens.long()]
+        return be.paged.append(x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:], k_pages, v_pages, pages, lengths, row_starts, inv, prefix_length=ahead,
+                               interleaved=interleaved)
+
+    put(ints(text), prefix[None], ints([prompt]), ints([0, prompt]), 0)
+    written, rnd = [1] * B, torch.Generator().manual_seed(0)
+    row_starts = torch.arange(0, B * (K + 1) + 1, K + 1, dtype=torch.int32, device=cuda)
+    while min(written) < total:
+        right = torch.randint(0, K + 1, (B,), generator=rnd).tolist()
+        drafts = [[want[b][written[b] + i] if i != right[b] else (want[b][written[b] + i] + 1) % V for i in range(K)] if written[b] < total else [0] * K
+                  for b in range(B)]
+        agree = [next((i for i in range(K) if written[b] + i >= len(want[b]) or drafts[b][i] != want[b][written[b] + i]), K) for b in range(B)]
+        pas = ints([[want[b][written[b] - 1]] + drafts[b] for b in range(B)]).flatten()
+        lengths = ints([w + K for w in written])                         # rows: the tokens written, the last of them in this pass, and the drafts
+        q = put(pas, table, lengths, row_starts, prompt)
+        o = be.paged.attention(q, k_pages, v_pages, table, lengths, row_starts, prefix_pages=prefix, prefix_length=prompt)
+        probs = torch.softmax(1000 * (o.float().flatten(1) @ proj), -1).view(B, K + 1, V)
+        tokens, accepted = be.verify_tokens(ints(drafts), probs, torch.full((B, K + 1), 0.5, device=cuda))
+        for b in range(B):
+            if written[b] >= total:                                      # (a request that is done stays where it is)
+                continue
+            n = int(accepted[b])
+            assert n == agree[b], (b, written[b], drafts[b], want[b][written[b]:written[b] + K + 1], tokens[b].tolist())
+            assert tokens[b, :n + 1].tolist() == want[b][written[b]:written[b] + n + 1] and (tokens[b, n + 1:] == -1).all()
+            written[b] += n + 1
+    assert be.paged.attention_error(cuda) == 0
