@@ -83,6 +83,8 @@ def _paged(q, k_pages, v_pages, page_table, lengths, row_starts) -> _lib.Paged:
     if pages < 1 or kv_heads < 1 or q.shape[1] < 1 or q.shape[1] % kv_heads or q.shape[1] > 4096:
         raise _lib.B200Error(f"{q.shape[1]} query heads (at most 4096) must be a multiple of the {kv_heads} key heads of at least one page")
     _check_page_size(page_size)
+    if max(*q.shape, *k_pages.shape, *page_table.shape) > 0x7fffffff:
+        raise _lib.B200Error("sizes must fit 32 bits")
     return _lib.Paged(_lib.DTYPES[q.dtype], lengths.numel(), q.shape[0], q.shape[1], kv_heads, q.shape[2], pages, page_size, page_table.shape[1],
                       _lib.ptr(page_table), page_table.stride(0), _lib.ptr(lengths), _lib.ptr(row_starts), _lib.ptr(k_pages), _lib.ptr(v_pages),
                       *k_pages.stride()[:3])
@@ -109,8 +111,8 @@ def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Ten
     _lib.require_tensor("v", v, (q.dtype,), k.shape, q, packed=False)
     if k.stride() != v.stride() and k.numel() > 0:
         raise _lib.B200Error("k and v must have the same strides")
-    if c.head_dim > 2048 or prefix_length < 0:
-        raise _lib.B200Error("append takes heads of at most 2048 dims and a prefix of at least 0 rows")
+    if c.head_dim > 2048 or not 0 <= prefix_length <= 0x7fffffff:
+        raise _lib.B200Error("append takes heads of at most 2048 dims and a prefix of 0 to 2^31 - 1 rows")
     r = rope._rotary(positions, inv_freqs, c.head_dim, c.tokens, q, scaling_factor, magnitude, interleaved)
     if q_out is None:
         q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -144,8 +146,8 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
 
     ``q (tokens, heads, dim)``, positions already in it; heads of 64 or 128; float16 or bfloat16, scores, statistics and sums in fp32, probabilities
     rounded to the type for the second product; NaN and infinities reach the tokens that see them, and no other.  ``out`` may be ``q``.  ``scale``, 0 or more, is
-    ``dim ** -0.5`` unless given.  A token that sees no row gets zeros.  Rows behind a
-    length may hold anything; a page number outside the cache stands for rows of zeros.  At most 1024 requests."""
+    ``dim ** -0.5`` unless given.  A token that sees no row gets zeros; results of tokens outside ``row_starts`` are
+    not written (``append`` likewise).  Rows behind a length may hold anything; a page number outside the cache stands for rows of zeros.  At most 1024 requests."""
     if out is None and isinstance(q, torch.Tensor):
         y = _lib.ops().paged_attention(q, k_pages, v_pages, page_table, lengths, row_starts, prefix_pages, prefix_length, mask, scale,
                                        _errors.get(q.device.index))
@@ -156,8 +158,8 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
         raise _lib.B200Error(f"attention takes heads of 64 or 128 dims, not {c.head_dim}")
     if c.requests > 1024:
         raise _lib.B200Error(f"attention takes at most 1024 requests, not {c.requests}")
-    if prefix_length < 0 or (prefix_length > 0) and prefix_pages is None:
-        raise _lib.B200Error("prefix_length needs prefix_pages, and must not be negative")
+    if not 0 <= prefix_length <= 1 << 30 or prefix_length > 0 and prefix_pages is None:
+        raise _lib.B200Error("prefix_length needs prefix_pages, and must be 0 to 2^30 rows")
     if prefix_pages is not None:
         _lib.require_tensor("prefix_pages", prefix_pages, (torch.int32,), (None,), q)
         if prefix_pages.numel() * c.page_size < prefix_length:

@@ -58,14 +58,21 @@ def frequencies(rotary_dim: int, base: float = 10000.0, rope_scaling: Optional[d
     rs = rope_scaling or {}
     kind = rs.get("type") or rs.get("rope_type", "default")
     scaling = magnitude = 1.0
+    needs = dict(linear=("factor",), llama3=("factor",), yarn=("factor", "original_max_position_embeddings")).get(kind, ())
+    if any(not float(rs.get(n) or 0.0) > 0.0 for n in needs):
+        raise _lib.B200Error(f"rope_scaling of type {kind} needs {' and '.join(needs)}, positive")
     if kind == "linear":
         scaling = 1.0 / float(rs["factor"])
     elif kind == "llama3":
         lo, hi = float(rs.get("low_freq_factor", 1.0)), float(rs.get("high_freq_factor", 4.0))
+        if not hi > lo:
+            raise _lib.B200Error("high_freq_factor must be more than low_freq_factor")
         turns = float(rs.get("original_max_position_embeddings", 8192)) * f / (2 * math.pi)
         keep = ((turns - lo) / (hi - lo)).clamp(0.0, 1.0)
         f = f * (keep + (1.0 - keep) / float(rs["factor"]))
     elif kind == "yarn":
+        if not base > 1.0 or any(rs.get(n) is not None for n in ("mscale", "mscale_all_dim")) or not rs.get("truncate", True):
+            raise _lib.B200Error("yarn takes a base above 1, its magnitude by attention_factor, not mscale, and borders rounded outwards")
         factor, length = float(rs["factor"]), float(rs["original_max_position_embeddings"])
 
         def index(turns):                                 # of the pair that turns so often (not whole)
@@ -107,8 +114,8 @@ def rotate(x: torch.Tensor, positions: torch.Tensor, inv_freqs: torch.Tensor, *,
             return y
     _lib.require_tensor("x", x, tuple(_lib.DTYPES), (None, None, None), packed=False)
     tokens, heads, dim = x.shape
-    if dim > 2048 or heads > 65535:
-        raise _lib.B200Error("rotate takes heads of at most 2048 dims and at most 65535 of them")
+    if dim > 2048 or heads > 65535 or tokens > 0x7fffffff:
+        raise _lib.B200Error("rotate takes heads of at most 2048 dims, at most 65535 of them, and at most 2^31 - 1 tokens")
     if positions is None:
         raise _lib.B200Error("rotate needs positions")
     r = _rotary(positions, inv_freqs, dim, tokens, x, scaling_factor, magnitude, interleaved, inverse)

@@ -541,3 +541,18 @@ def test_speculation_writes_what_plain_steps_write(be, cuda, interleaved):
             assert tokens[b, :n + 1].tolist() == want[b][written[b]:written[b] + n + 1] and (tokens[b, n + 1:] == -1).all()
             written[b] += n + 1
     assert be.paged.attention_error(cuda) == 0
+
+
+def test_sizes_beyond_32_bits_are_refused(be, cuda):
+    """Not cut to what is left of them."""
+    b = Batch(cuda, 4, 2, 64, 16, 20, [14, 0], [4, 2])
+    inv, _, _ = be.rope.frequencies(64, device=cuda)
+    k = torch.randn(6, 2, 64, device=cuda).half()
+    base = [b.k_pages, b.v_pages, b.table, b.lengths, b.row_starts]
+    far = (1 << 32) + 5
+    calls = [lambda: be.paged.append(b.q, k, k, *base, inv, prefix_length=far), lambda: be.paged.attention(b.q, *base, prefix_pages=b.prefix_pages, prefix_length=far),
+             lambda: be.paged.append(b.q[:1].expand(far, 4, 64), k[:1].expand(far, 2, 64), k[:1].expand(far, 2, 64), *base, inv),
+             lambda: be.rope.rotate(b.q[:1].expand(far, 4, 64), torch.zeros(6, device=cuda).int(), inv)]
+    for call in calls:
+        with pytest.raises(be._lib.B200Error):
+            call()

@@ -64,7 +64,8 @@ def test_attention_entry(be):
     assert lib.b200_paged_attention_workspace_bytes(ctypes.byref(_cache(be, base, kv_heads=3))) == 0
     for kw in (dict(head_dim=96), dict(page_size=12), dict(page_size=4), dict(page_size=192)):
         assert call(_cache(be, base, **kw)) == -1, kw
-    assert call(_cache(be, base, requests=1025)) == -6
+    assert call(_cache(be, base, requests=1025)) == call(_cache(be, base, table_width=(1 << 26) + 1)) == -6
+    assert call(_cache(be, base), prefix=base, length=(1 << 30) + 1) == call(_cache(be, base), prefix=base, length=0x7fffffff) == -6
     assert call(_cache(be, base), length=5) == call(_cache(be, base), prefix=base, length=-1) == -1
     assert call(_cache(be, base), q=None) == call(_cache(be, base), ws=None) == call(_cache(be, base), error=None) == -1
     assert call(_cache(be, base), scale=-1.0) == call(_cache(be, base), scale=float("nan")) == -1
@@ -93,6 +94,17 @@ def test_no_cpu_path(be):
                  lambda: be.paged.attention(x, pages, pages, table, n, starts), lambda: be.verify_tokens(table, torch.zeros(1, 3, 8), torch.zeros(1, 3))):
         with pytest.raises(be._lib.B200Error, match="CUDA"):
             call()
+
+
+def test_scalings_that_are_not_known_are_refused(be):
+    yarn = dict(type="yarn", factor=4.0, original_max_position_embeddings=4096)
+    assert be.rope.frequencies(64, 1e4, yarn)[2] > 1.0
+    for bad in (dict(type="linear"), dict(type="linear", factor=0.0), dict(type="llama3"), dict(type="llama3", factor=8.0, low_freq_factor=4.0),
+                dict(type="yarn", factor=4.0), dict(yarn, factor=-1.0), dict(yarn, mscale=0.7), dict(yarn, truncate=False), dict(type="longrope", factor=2.0)):
+        with pytest.raises(be._lib.B200Error):
+            be.rope.frequencies(64, 1e4, bad)
+    with pytest.raises(be._lib.B200Error):
+        be.rope.frequencies(64, 1.0, yarn)
 
 
 def test_pages_of_the_pool_are_handed_out_once(be):
