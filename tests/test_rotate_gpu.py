@@ -156,3 +156,29 @@ def test_rotate_refusals(be, cuda):
     for call in calls:
         with pytest.raises(E):
             call()
+
+
+def test_calls_on_two_streams_and_replayed(be, cuda):
+    """Rotations side by side and from a graph, with positions that change: the same bits as one call after the other."""
+    inv, _, _ = be.rope.frequencies(128, device=cuda)
+    xs = [torch.randn(n, 6, 128, device=cuda).half() for n in (1, 300, 3000)]
+    pos = [torch.arange(7, 7 + x.shape[0], device=cuda) for x in xs]
+    want = [be.rope.rotate(x, p, inv) for x, p in zip(xs, pos)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(3):
+        for i, (x, p) in enumerate(zip(xs, pos)):
+            got.append((i, be.rope.rotate(x, p, inv)))
+            with torch.cuda.stream(side):
+                got.append((i, be.rope.rotate(x, p, inv)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, y in got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [be.rope.rotate(x, p, inv) for x, p in zip(xs, pos)]
+    for p in pos:
+        p += 1000
+    graph.replay()
+    assert all(torch.equal(y, be.rope.rotate(x, p, inv)) for x, p, y in zip(xs, pos, out))
+    assert not torch.equal(out[1], want[1])
