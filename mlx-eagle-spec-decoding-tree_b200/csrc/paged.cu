@@ -19,7 +19,7 @@
 //
 // What bounds it: for pairs the chain of products, softmax and waits (4240 cycles a block of 256 rows, 2144 of them products: 16 x 64 tokens of 32
 // heads behind 32768 rows 505 us, 1.1 PFLOP/s, and 580 at the power limit); for single streams the copies (64 x 1 tokens behind 16384 rows, 1024 rows
-// each: 66 us, 3.2 TB/s), and where they are short the start and the join, some 10 us.
+// each: 65 us, 3.2 TB/s), and where they are short the start and the join, some 10 us.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -105,7 +105,7 @@ struct Request {
 };
 __device__ __forceinline__ Request request_of(const PagedParams& p, int b) {
     Request r;
-    const int s0 = p.row_starts[b], s1 = p.row_starts[b + 1], len = p.lengths[b];
+    const int s0 = __ldcg(p.row_starts + b), s1 = __ldcg(p.row_starts + b + 1), len = __ldcg(p.lengths + b);
     r.start = min(max(s0, 0), p.tokens);
     r.count = min(max(s1 - r.start, 0), p.tokens - r.start);
     r.length = (int)min((long long)max(len, 0), (long long)p.table_width * p.page_size);
@@ -314,8 +314,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     const uint32_t tmem = s_tmem;
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();                                             // (behind the wait: the join reads row_starts and lengths before it waits itself)
     // (what earlier kernels wrote by ordinary stores, rows and queries: 2000 cycles, of which all but a few pass behind the scan below)
     if (warp == kKeyLoader || warp == kValueLoader) asm volatile("fence.proxy.async;\n" ::: "memory");
 
@@ -749,21 +749,27 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
 // their loads in flight.  (512 rows of 16 requests behind 16384 rows: attention in 29.6 us, by one warp a row 32.9; 2048 rows of 64: 60.4 and
 // 58.0.)
 template <typename T, int HD, int WAYS>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedParams p, int ctas) {
+__global__ void __launch_bounds__(128, 8) paged_join_kernel(const __grid_constant__ PagedParams p, int ctas) {
     pdl_launch_dependents();
-    pdl_wait();
     constexpr int N = HD / 32, BATCH = 4;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = WAYS == 1 ? blockIdx.y * 4 + warp : blockIdx.y, t = blockIdx.x, way = WAYS == 1 ? 0 : warp;
-    if (head >= p.heads) return;
-    if (t < p.row_starts[0] || t >= p.row_starts[p.requests]) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = blockIdx.x;
+    const int head = WAYS == 1 ? blockIdx.y * 4 + warp : blockIdx.y, way = WAYS == 1 ? 0 : warp;
+    // Whose token it is does not depend on the attention, which starts this kernel only once all ahead of it is there: these reads pass while its
+    // last CTAs work (64 requests behind 16384 rows 58.2 -> 56.6 us, 4 short ones 11.3 -> 10.7, though 557 -> 566 where the join has 32768 rows).  Who
+    // has nothing to do waits all the same: a kernel behind this one must not start ahead of the attention's end.
+    if (head >= p.heads || t < __ldcg(p.row_starts) || t >= __ldcg(p.row_starts + p.requests)) {
+        pdl_wait();
+        return;
+    }
     int lo = 0, hi = p.requests;
     while (hi - lo > 1) {
         const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
-        const int n = __popc(__ballot_sync(0xffffffffu, at < hi && p.row_starts[at] <= t));
+        const int n = __popc(__ballot_sync(0xffffffffu, at < hi && __ldcg(p.row_starts + at) <= t));
         lo += n * step;
         hi = min(hi, lo + step);
     }
     const Request q = request_of(p, lo);
+    pdl_wait();
     const Line& l = p.line;
     const int singles = p.plan[p.requests + 1];
     const Share single(l.odd + p.plan[p.requests], 2 * singles);
