@@ -279,7 +279,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
     __shared__ long long s_warp[kPgThreads / 32];
     __shared__ Cursor s_from[2];                                         // of either stream; the first's for both of a pair
     __shared__ int s_segments;
-    __shared__ float s_part[2][2][kParts][kRows];                        // [stream][in turn]: what a row's threads tell one another
+    __shared__ float s_part[2][2][kParts][kRows];                        // [stream][in turn]: the maxima that a row's threads tell one another
+    __shared__ float s_sum[2][kRows];                                    // of a piece, from the row's second thread to its first
     const uint32_t sbase = smem_u32(smem);
     const int lane = threadIdx.x & 31, warp = uniform(threadIdx.x >> 5), ctas = gridDim.x, cta = blockIdx.x;
 
@@ -669,10 +670,11 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
             __syncwarp();
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             if (busy) {
-                float l = sum;
-                s_part[s][blocks & 1][part][r] = l;                      // (not where the last block's maximum was)
+                // (in a place of their own: a partner held up behind this barrier reads while the next piece's first maxima are written, and its next
+                // sum is written behind their barrier)
+                if (part == 1) s_sum[s][r] = sum;
                 row_sync();
-                l += s_part[s][blocks & 1][part ^ 1][r];
+                const float l = sum + s_sum[s][r];                       // (used by the first)
                 const long long row = (long long)t * p.heads + c.hk * p.group + g, all = (long long)p.tokens * p.heads;
                 float* dst;
                 long long at;

@@ -556,3 +556,14 @@ def test_sizes_beyond_32_bits_are_refused(be, cuda):
     for call in calls:
         with pytest.raises(be._lib.B200Error):
             call()
+
+
+@pytest.mark.parametrize("shape", [(8, 4, 128), (14, 2, 64)], ids=str)
+def test_workers_of_many_pieces(be, cuda, shape):
+    """Segments of a block or two, a dozen to a worker: the sum of a piece and the maxima of the next, which begins at once, are told apart, so that
+    every run gives the same bits, those of the definition."""
+    n = 900
+    b = Batch(cuda, *shape, 16, 40, [(37 * i) % 200 for i in range(n)], [1 + i % 3 for i in range(n)])
+    want = b.check(be)
+    for _ in range(30):
+        assert torch.equal(b.run(be), want)
