@@ -948,9 +948,11 @@ __global__ void __launch_bounds__(128, 8) paged_join_kernel(const __grid_constan
 }
 
 struct Room {
-    size_t prefix, own, behind, pair, more, ml, plan, total;             // byte offsets
+    size_t prefix, own, behind, pair, more, ml, plan, total;             // byte offsets from the workspace's first place for them
     int ctas;
 };
+// Pieces are stored 32 bytes at a time; a workspace begins at a multiple of 16.
+constexpr size_t kWorkAlign = 32, kGivenAlign = 16;
 Room room_of(const b200_paged* c, int ctas) {
     Room r{};
     const size_t all = (size_t)c->tokens * c->heads, row = (size_t)c->head_dim * 4, pair = (size_t)ctas * 2 * kRows, more = (size_t)2 * ctas * kRows;
@@ -962,7 +964,7 @@ Room room_of(const b200_paged* c, int ctas) {
     r.ml = r.more + more * row;
     r.plan = r.ml + (3 * all + pair + more) * sizeof(float2);
     r.total = r.plan + (c->requests + 2) * sizeof(int);
-    r.total = (r.total + 15) / 16 * 16;
+    r.total = (r.total + 15) / 16 * 16 + (kWorkAlign - kGivenAlign);
     return r;
 }
 int grid_ctas() {
@@ -1054,7 +1056,7 @@ int b200_paged_attention(const b200_paged* c, const void* q, long long q_token, 
         if (rc != B200_OK) return rc;
     }
     const Room r = room_of(c, 148);
-    char* ws = static_cast<char*>(workspace);
+    char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(workspace) + kWorkAlign - 1) / kWorkAlign * kWorkAlign);
     p.first_prefix = reinterpret_cast<float*>(ws + r.prefix); p.first_own = reinterpret_cast<float*>(ws + r.own);
     p.first_behind = reinterpret_cast<float*>(ws + r.behind);
     p.more_pair = reinterpret_cast<float*>(ws + r.pair); p.more = reinterpret_cast<float*>(ws + r.more);

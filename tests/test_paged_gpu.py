@@ -6,6 +6,7 @@ S = scale * sum |q k| (128 terms, 2^-24 each, and as much again for a sum that t
 relatively (its own and the sum's), as do the roundings of exp2 and of the running sums, 2^-18 together for up to 2^14 rows.  fp16
 probabilities below 2^-14 are off by up to 2^-25 in place of e p, relative to the largest: a row of n keys by n 2^-25 max |v| at most, over a sum of
 at least 1."""
+import ctypes
 import math
 
 import pytest
@@ -567,3 +568,20 @@ def test_workers_of_many_pieces(be, cuda, shape):
     want = b.check(be)
     for _ in range(30):
         assert torch.equal(b.run(be), want)
+
+
+@pytest.mark.parametrize("ahead", [0, 16, 32, 48])
+def test_a_workspace_may_begin_at_any_16_bytes(be, cuda, ahead):
+    """By the C entry, in just the bytes that it asks for: the same bits wherever it begins, and nothing behind it is written."""
+    b = Batch(cuda, 8, 2, 128, 16, 1500, [700, 90, 0], [3, 140, 1])
+    want = b.check(be)
+    lib, ptr = be._lib.lib(), be._lib.ptr
+    c = be.paged._paged(b.q, b.k_pages, b.v_pages, b.table, b.lengths, b.row_starts)
+    room = lib.b200_paged_attention_workspace_bytes(ctypes.byref(c))
+    ws = torch.full((room + 128,), 113, dtype=torch.uint8, device=cuda)
+    assert ws.data_ptr() % 64 == 0
+    out, err = torch.empty_like(b.q), torch.zeros(1, dtype=torch.int32, device=cuda)
+    rc = lib.b200_paged_attention(ctypes.byref(c), ptr(b.q), *b.q.stride()[:2], ptr(out), *out.stride()[:2], ptr(b.prefix_pages), b.prefix, None,
+                                  128 ** -0.5, ptr(ws[ahead:]), room, ptr(err), be._lib.stream_ptr(cuda))
+    assert rc == 0 and torch.equal(out, want) and int(err) == 0
+    assert (ws[:ahead] == 113).all() and (ws[ahead + room:] == 113).all()
