@@ -188,6 +188,7 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
 
 
 def attention_error(device) -> int:
-    """Non-zero if a bounded wait inside an attention on this device ever ran out (reads the flag)."""
-    word = _errors.get(torch.device(device).index)
+    """Non-zero if a bounded wait inside an attention on this device (without an index: the current one) ever ran out (reads the flag)."""
+    device = torch.device(device)
+    word = _errors.get(torch.cuda.current_device() if device.index is None and _errors else device.index)
     return 0 if word is None else int(word.item())

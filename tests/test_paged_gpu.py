@@ -585,3 +585,17 @@ def test_a_workspace_may_begin_at_any_16_bytes(be, cuda, ahead):
                                   128 ** -0.5, ptr(ws[ahead:]), room, ptr(err), be._lib.stream_ptr(cuda))
     assert rc == 0 and torch.equal(out, want) and int(err) == 0
     assert (ws[:ahead] == 113).all() and (ws[ahead + room:] == 113).all()
+
+
+def test_the_error_word_is_read_back(be, cuda):
+    """Set by the host, in the place of a wait that ran out, and found by every name of the device."""
+    b = Batch(cuda, 4, 2, 64, 16, 20, [14, 0], [4, 2])
+    b.run(be)
+    word = be.paged._errors[b.q.device.index]
+    try:
+        word.fill_(31)
+        for name in ("cuda", torch.device("cuda"), b.q.device.index, f"cuda:{b.q.device.index}", b.q.device):
+            assert be.paged.attention_error(name) == 31
+    finally:
+        word.zero_()
+    b.check(be)

@@ -120,3 +120,15 @@ def test_pages_of_the_pool_are_handed_out_once(be):
         with pytest.raises(be._lib.B200Error):
             cache.give(pages)
     assert cache.layer(0)[0].shape == (6, 2, 16, 64)
+
+
+def test_the_error_word_is_found_however_its_device_is_named(be, monkeypatch):
+    monkeypatch.setattr(be.paged, "_errors", {0: torch.tensor([31], dtype=torch.int32), 1: torch.tensor([0], dtype=torch.int32)})
+    for current, words in ((0, 31), (1, 0)):
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: current)
+        assert be.paged.attention_error("cuda") == be.paged.attention_error(torch.device("cuda")) == words
+    for name in (0, "cuda:0", torch.device("cuda", 0)):
+        assert be.paged.attention_error(name) == 31
+    assert be.paged.attention_error("cuda:1") == be.paged.attention_error("cuda:2") == 0
+    monkeypatch.setattr(be.paged, "_errors", {})
+    assert be.paged.attention_error("cuda") == 0
