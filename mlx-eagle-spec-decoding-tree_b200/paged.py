@@ -133,7 +133,9 @@ def _error_word(device) -> torch.Tensor:
     if word is None:
         if torch.cuda.is_current_stream_capturing():
             raise _lib.B200Error("the first attention on a device must not be captured: its error word would belong to the graph")
-        word = _errors[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+        word = torch.zeros(1, dtype=torch.int32, device=device)
+        torch.cuda.current_stream(device).synchronize()                  # (other streams set it and read it)
+        _errors[device.index] = word
     return word
 
 

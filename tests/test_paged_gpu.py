@@ -599,3 +599,23 @@ def test_the_error_word_is_read_back(be, cuda):
     finally:
         word.zero_()
     b.check(be)
+
+
+def test_the_error_word_is_clear_for_every_stream(be, cuda, monkeypatch):
+    """Made by a call on a stream that has work ahead of it, and read on another at once: its zero is there, not what the memory held."""
+    b = Batch(cuda, 4, 2, 64, 16, 20, [14, 0], [4, 2])
+    want = b.run(be)
+    monkeypatch.setattr(be.paged, "_errors", {})
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        used = torch.full((1,), 77, dtype=torch.int32, device=cuda)      # (the allocator's next block of this size)
+        torch.cuda.current_stream().synchronize()
+        del used
+        torch.cuda._sleep(40_000_000)                                    # 20 ms
+        be.paged._error_word(b.q.device)                                 # (as the first attention does)
+    assert be.paged.attention_error(b.q.device) == 0
+    with torch.cuda.stream(side):
+        got = b.run(be)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
