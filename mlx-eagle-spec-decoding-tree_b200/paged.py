@@ -189,8 +189,14 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     return out
 
 
-def attention_error(device) -> int:
-    """Non-zero if a bounded wait inside an attention on this device (without an index: the current one) ever ran out (reads the flag)."""
+def attention_error(device, clear: bool = False) -> int:
+    """Non-zero if a bounded wait inside an attention on this device (without an index: the current one) ever ran out, or ran out since the word
+    was cleared (reads the flag, in the order of the current stream)."""
     device = torch.device(device)
     word = _errors.get(torch.cuda.current_device() if device.index is None and _errors else device.index)
-    return 0 if word is None else int(word.item())
+    found = 0 if word is None else int(word.item())
+    if clear and found:
+        word.zero_()
+        if word.is_cuda:
+            torch.cuda.current_stream(word.device).synchronize()
+    return found

@@ -619,3 +619,25 @@ def test_the_error_word_is_clear_for_every_stream(be, cuda, monkeypatch):
         got = b.run(be)
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("prefix,old,new", [(20000, [100, 2500], [1, 1]), (3000, [5, 5], [300, 400])])
+def test_a_short_wait_limit_changes_no_result_and_the_error_word_clears(be, cuda, prefix, old, new):
+    """A limit of one poll, for calls and captured ones.  (A poll takes some 4 us, and all that a wait here is for comes within two, so that the word stays
+    clear by itself: the host sets it.)"""
+    lib = be._lib.lib()
+    b = Batch(cuda, 8, 2, 128, 16, prefix, old, new)
+    want = b.check(be)
+    word, graph = be.paged._errors[b.q.device.index], torch.cuda.CUDAGraph()
+    try:
+        lib.b200_set_wait_limit(1)
+        word.fill_(31)
+        assert torch.equal(b.run(be), want)
+        with torch.cuda.graph(graph):
+            got = b.run(be)
+    finally:
+        lib.b200_set_wait_limit(0)
+    graph.replay()
+    assert torch.equal(got, want)
+    assert be.paged.attention_error(cuda) == be.paged.attention_error(cuda, clear=True) == 31 and be.paged.attention_error(cuda) == 0
+    b.check(be)

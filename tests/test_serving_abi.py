@@ -130,5 +130,6 @@ def test_the_error_word_is_found_however_its_device_is_named(be, monkeypatch):
     for name in (0, "cuda:0", torch.device("cuda", 0)):
         assert be.paged.attention_error(name) == 31
     assert be.paged.attention_error("cuda:1") == be.paged.attention_error("cuda:2") == 0
+    assert be.paged.attention_error(0, clear=True) == 31 and be.paged.attention_error(0) == 0
     monkeypatch.setattr(be.paged, "_errors", {})
     assert be.paged.attention_error("cuda") == 0
