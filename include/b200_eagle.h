@@ -507,8 +507,8 @@ int b200_kv_compact(void* cache, int layers, int Hkv, int cache_rows, int hd, co
  * ------------------------------------------------------------------------------------------ */
 
 /* Rotation by theta = position * scaling * inv_freqs[i]: (a, b) -> magnitude * (a cos - b sin, a sin + b cos) for the pairs (x[i],
- * x[i + rotary_dim / 2]) or, interleaved, (x[2 i], x[2 i + 1]).  Dims from rotary_dim on pass through.  The angle is the product of the
- * numbers given, whatever the position: it is reduced to a turn in whole numbers. */
+ * x[i + rotary_dim / 2]) or, interleaved, (x[2 i], x[2 i + 1]).  Dims from rotary_dim on pass through.  The angle is reduced to a
+ * turn in whole numbers: that of the numbers given to within 2^-24 radians up to 2^37 rows, twice that for every doubling beyond. */
 typedef struct b200_rotary {
     const void* positions;      /* [tokens] int32, or int64 */
     const float* inv_freqs;     /* [rotary_dim / 2] */

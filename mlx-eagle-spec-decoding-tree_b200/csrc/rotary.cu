@@ -5,13 +5,15 @@
 // for the pairs (x[i], x[i + R/2]) or, interleaved, (x[2i], x[2i + 1]) of the first R dims; the dims behind them pass through.
 //
 // The angle is reduced in whole numbers: scaling * inv_freq / 2 pi as a 64-bit fraction of a turn, times the position modulo 2^64, is the
-// fraction of a turn of the product, whatever the position (53 bits of the product of doubles: 2^-37 turns at 131072 and a frequency of
-// one, where a product in single precision is off by 2^-9 radians).  Products and sums of a pair are fp32, rounded once to the result's type.
+// fraction of a turn of the product.  The fraction comes from a product in two doubles each and is off by 2^-64 at most, so the angle by 2^-24
+// radians, fp32's own step, at 2^37 rows (2^-44 at 131072, where a product in single precision is off by 2^-9; one double's 53 bits left 2.4e-7 radians at
+// 2^31 and 1.2e-4 at 2^40).  Products and sums of a pair are fp32, rounded once to the result's type.
 //
 // A CTA has a token or two: its threads turn the angles once (the only costly arithmetic), then all go over the heads, 16 bytes an item, two in
-// flight.  What bounds it: instructions (address, conversion) and the wait for the angles; 4099 tokens of 32 x 128 16-bit elements 13.2 us (5.1 TB/s, 77 %
-// of a copy's rate), ragged prompts with their scattered rows 49.3 (4.3 TB/s, 65 %), one token 3.9 (the launch).
+// flight.  What bounds it: instructions (address, conversion) and the wait for the angles; 4099 tokens of 32 x 128 16-bit elements 13.3 us (5.0 TB/s, 77 %
+// of a copy's rate; 13.2 with the fraction from one double), ragged prompts 49.4 (4.3 TB/s, 65 %; 49.3), one token 3.9 (the launch).
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -39,7 +41,7 @@ struct RotParams {
     const void* positions;                       // or NULL: row in the request, behind the prefix
     int pos64;
     const float* inv_freqs;
-    double turns;                                // scaling / 2 pi
+    double turns, turns_low;                     // scaling / 2 pi, and what its rounding left
     float magnitude;
     int inverse;
     int tokens, heads, kv_heads, dim, half;      // half: pairs that are rotated
@@ -64,9 +66,9 @@ __device__ __forceinline__ int find_request(const int* starts, int requests, int
 
 // magnitude * (cos, sin) of frequency i at a position.
 __device__ __forceinline__ float2 turn_of(const RotParams& p, int i, long long pos) {
-    double f = p.inv_freqs[i] * p.turns;
-    f -= floor(f);
-    const unsigned long long phase = __double2ull_rz(f * 0x1p64) * (unsigned long long)pos;
+    const double f = p.inv_freqs[i], high = f * p.turns, low = fma(f, p.turns_low, fma(f, p.turns, -high));
+    const unsigned long long fraction = (unsigned long long)__double2ll_rn((high - rint(high)) * 0x1p64) + (unsigned long long)__double2ll_rn(low * 0x1p64);
+    const unsigned long long phase = fraction * (unsigned long long)pos;
     const unsigned quarter = (unsigned)((phase + (1ull << 61)) >> 62);                       // the nearest quarter of a turn, what is left to either side
     float s, c;
     sincospif((float)(long long)(phase - ((unsigned long long)quarter << 62)) * 0x1p-63f, &s, &c);
@@ -256,7 +258,12 @@ int launch_rotary(RotParams& p, bool interleaved, cudaStream_t stream) {
     return check_launch();
 }
 
-constexpr double kTwoPi = 6.283185307179586476925286766559;
+// 1 / 2 pi, and what its rounding left.
+constexpr double kTurn = 0x1.45f306dc9c883p-3, kTurnLow = -0x1.6b01ec5417056p-57;
+void set_turns(RotParams& p, double scaling) {
+    p.turns = scaling * kTurn;
+    p.turns_low = std::fma(scaling, kTurn, -p.turns) + scaling * kTurnLow;
+}
 
 }  // namespace
 }  // namespace b200
@@ -273,7 +280,7 @@ int b200_rotate(const b200_rotary* r, const void* x, long long x_token, long lon
     b200::RotParams p{};
     p.in = {static_cast<char*>(const_cast<void*>(x)), x_token, x_head};
     p.out = {static_cast<char*>(out), out_token, out_head};
-    p.positions = r->positions; p.pos64 = r->positions_64; p.inv_freqs = r->inv_freqs; p.turns = r->scaling / b200::kTwoPi;
+    p.positions = r->positions; p.pos64 = r->positions_64; p.inv_freqs = r->inv_freqs; b200::set_turns(p, r->scaling);
     p.magnitude = r->magnitude; p.inverse = r->inverse; p.tokens = tokens; p.heads = heads; p.dim = dim; p.half = r->rotary_dim / 2;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == B200_DTYPE_F32) return b200::launch_rotary<float, false>(p, r->interleaved, st);
@@ -295,7 +302,7 @@ int b200_paged_append(const b200_paged* c, const b200_rotary* r, const void* q, 
     p.out = {static_cast<char*>(q_out), out_token, out_head};
     p.k_pages = static_cast<char*>(c->k_pages); p.v_pages = static_cast<char*>(c->v_pages);
     p.page_stride = c->page_stride; p.page_head = c->head_stride; p.page_row = c->row_stride;
-    p.positions = r->positions; p.pos64 = r->positions_64; p.inv_freqs = r->inv_freqs; p.turns = r->scaling / b200::kTwoPi;
+    p.positions = r->positions; p.pos64 = r->positions_64; p.inv_freqs = r->inv_freqs; b200::set_turns(p, r->scaling);
     p.magnitude = r->magnitude;
     p.tokens = c->tokens; p.heads = c->heads; p.kv_heads = c->kv_heads; p.dim = c->head_dim; p.half = r->rotary_dim / 2;
     p.table = c->page_table; p.lengths = c->lengths; p.row_starts = c->row_starts; p.table_stride = c->table_stride;

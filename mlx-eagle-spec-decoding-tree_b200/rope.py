@@ -7,8 +7,8 @@ non-traditional (element i pairs with i + D/2), math in fp32, output in the inpu
 dtype.  Inside the decode loop the same rotation runs fused with the KV-cache
 append (``b200_rope_kv_append``); this stand-alone form is the drop-in operator.
 
-``rotate`` is the general form: either order of the pairs, part of the head, 16- and 32-bit types, strided rows, angles that stay exact at
-far positions, and the inverse.  ``frequencies`` gives its frequencies for plain models and for ones stretched to longer contexts.
+``rotate`` is the general form: either order of the pairs, part of the head, 16- and 32-bit types, strided rows, angles that keep
+fp32's precision at far positions, and the inverse.  ``frequencies`` gives its frequencies for plain models and for ones stretched to longer contexts.
 """
 from __future__ import annotations
 
@@ -104,7 +104,7 @@ def rotate(x: torch.Tensor, positions: torch.Tensor, inv_freqs: torch.Tensor, *,
     """``x (tokens, heads, dim)`` rotated by ``positions (tokens,)`` times ``scaling_factor * inv_freqs``: the pairs ``(x[i], x[i + R/2])``, or
     ``interleaved`` ``(x[2i], x[2i + 1])``, of the first ``R = 2 * len(inv_freqs)`` dims become ``magnitude * (a cos - b sin, a sin + b cos)``; the rest
     passes through.  float16, bfloat16 or float32, fp32 inside, rounded once; tokens and heads may be strided (a slice of a fused
-    projection).  Positions are int32 or int64, angles exact to the last bit that matters at any of them.
+    projection).  Positions are int32 or int64; an angle is off by less than 2^-24 radians, fp32's own step, up to 2^37 rows, and by twice that a doubling beyond.
 
     ``inverse`` rotates by the negative angle: the gradient of a rotation with respect to ``x`` is the rotation of the result's gradient
     with ``inverse`` and the same magnitude.  ``out`` may be ``x`` itself; other overlaps are undefined.  No gradient is recorded."""

@@ -3,6 +3,9 @@
 Tolerance: of a rotated pair (a, b), magnitude m: the angle is off by at most 2^-25 (its fraction of a turn rounded to fp32 in an eighth of a turn to
 either side), sine and cosine by two units of 2^-24, m times them, two products and their sum by half a unit each: below 2^-21 m (|a| + |b|)
 in all, and the result's rounding: half a step of its type, or of the smallest fp16 numbers, 2^-25."""
+import math
+from fractions import Fraction
+
 import pytest
 import torch
 
@@ -182,3 +185,20 @@ def test_calls_on_two_streams_and_replayed(be, cuda):
     graph.replay()
     assert all(torch.equal(y, be.rope.rotate(x, p, inv)) for x, p, y in zip(xs, pos, out))
     assert not torch.equal(out[1], want[1])
+
+
+def test_positions_beyond_32_bits_keep_their_angles(be, cuda):
+    """Against angles reduced in fractions of 80 digits.  Up to 2^37 rows an angle is off by 2^-24 more than near ones (half of 2^-23), where the tolerance has
+    room: 2^-25 + 2 units of 2^-24, 2 products and a sum make 1.75 x 2^-23 (and 0.5 now) of the 4 x 2^-23 that it is."""
+    turn = Fraction(1) / (2 * Fraction("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899"))
+    pos = [p + d for p in (1 << 31, 1 << 34, (1 << 37) - 3000, -(1 << 36)) for d in (-1, 0, 777, 2049)]
+    x = torch.randn(len(pos), 2, 128, generator=torch.Generator().manual_seed(2)).to(cuda)
+    inv, _, _ = be.rope.frequencies(128, 5e5)
+    for scaling in (1.0, 1 / 3):
+        angle = torch.empty(len(pos), 64, dtype=torch.float64)
+        for j, f in enumerate(inv.tolist()):
+            for i, p in enumerate(pos):
+                angle[i, j] = 2 * math.pi * float(Fraction(f) * Fraction(scaling) * p * turn % 1)
+        c, s, (a, b) = angle.cos().to(cuda)[:, None], angle.sin().to(cuda)[:, None], x.double().chunk(2, -1)
+        size = (a.abs() + b.abs()).repeat(1, 1, 2)
+        close(be.rope.rotate(x, torch.tensor(pos, device=cuda), inv.to(cuda), scaling_factor=scaling), torch.cat([a * c - b * s, a * s + b * c], -1), size, F32)
