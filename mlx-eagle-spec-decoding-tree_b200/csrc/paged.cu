@@ -847,11 +847,13 @@ __global__ void __launch_bounds__(128, 8) paged_join_kernel(const __grid_constan
                     x = p.ml[pick(seg[0].more_ml, seg[1].more_ml, seg[2].more_ml) + at];
                 }
             }
+            // (all of them, those of weight 0 too: 0 x Inf or NaN is NaN, wherever the line was cut)
+            unsigned left = __ballot_sync(0xffffffffu, src != nullptr);
+            if (left == 0) continue;
             float top = x.x;
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            if (top == -INFINITY) continue;                                  // (the same in all lanes)
-            const float high = fmaxf(m, top), before = exp2_approx(m - high), weight = x.x == -INFINITY ? 0.f : exp2_approx(x.x - high);
+            const float high = fmaxf(m, top), before = m == high ? 1.f : exp2_approx(m - high), weight = x.x == -INFINITY ? 0.f : exp2_approx(x.x - high);
             float l2 = weight * x.y;
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) l2 += __shfl_xor_sync(0xffffffffu, l2, d);
@@ -859,7 +861,6 @@ __global__ void __launch_bounds__(128, 8) paged_join_kernel(const __grid_constan
             m = high;
 #pragma unroll
             for (int e = 0; e < N; e++) o[e] *= before;
-            unsigned left = __ballot_sync(0xffffffffu, weight > 0.f || weight != weight);      // (NaN: scores of NaN make the row NaN)
             while (left) {
                 float w[BATCH];
                 Vec<float, N> v[BATCH];
@@ -869,8 +870,8 @@ __global__ void __launch_bounds__(128, 8) paged_join_kernel(const __grid_constan
                     const float* from = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), j));
                     w[b] = __shfl_sync(0xffffffffu, weight, j);
                     if (left) load_vec<true>(v[b], from + lane * N, N);
-                    else w[b] = 0.f;
-                    if (w[b] == 0.f)
+                    else w[b] = -1.f;
+                    if (w[b] < 0.f)                                          // (none; by a test on `left` the code came out 0.4 us a call slower)
 #pragma unroll
                         for (int e = 0; e < N; e++) v[b].v[e] = 0.f;
                     left &= left - 1;
@@ -897,8 +898,7 @@ __global__ void __launch_bounds__(128, 8) paged_join_kernel(const __grid_constan
             for (int e = 0; e < N; e++) o[e] = 0.f;
 #pragma unroll
             for (int w = 0; w < WAYS; w++) {                                 // (in order: the same bits every time)
-                if (s_m[w] == -INFINITY) continue;
-                const float a = exp2_approx(s_m[w] - m);
+                const float a = s_m[w] == m ? 1.f : exp2_approx(s_m[w] - m);
                 sum += a * s_sum[w];
 #pragma unroll
                 for (int e = 0; e < N; e++) o[e] += a * s_o[w][lane * N + e];

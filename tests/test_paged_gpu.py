@@ -641,3 +641,26 @@ def test_a_short_wait_limit_changes_no_result_and_the_error_word_clears(be, cuda
     assert torch.equal(got, want)
     assert be.paged.attention_error(cuda) == be.paged.attention_error(cuda, clear=True) == 31 and be.paged.attention_error(cuda) == 0
     b.check(be)
+
+
+@pytest.mark.parametrize("prefix,old,new", [(20000, [3], [1]), (2000, [100, 3], [40, 2]), (900, [7] * 20, [30] * 20)])
+def test_values_of_weights_that_are_too_small_for_a_number_reach_the_row(be, cuda, prefix, old, new):
+    """The prefix's scores lie 144 below the own rows', so that its weights are 0: its NaN and infinities make NaN of a row's dims all the same, whichever
+    piece of the line they are in, and the other dims are what the own rows make them."""
+    b = Batch(cuda, 8, 2, 64, 16, prefix, old, new)
+    own = Batch(cuda, 8, 2, 64, 16, 0, old, new)
+    b.q.fill_(3.0)
+    b.shared[0] = -3.0
+    for r, o in zip(b.rows, own.rows):
+        r[0] = 3.0
+        o.copy_(r)
+    own.q = b.q
+    b.shared[1, 0, 0, 5], b.shared[1, 0, prefix // 2, 9], b.shared[1, 1, prefix - 1, 11] = math.nan, math.inf, -math.inf
+    b._put(b.prefix_pages.tolist(), b.shared)
+    for i, r in enumerate(b.rows):
+        b._put(b.table[i].tolist(), r)
+    got = b.run(be)
+    want, tol = own.exact()
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[:, :4, 5] = hit[:, :4, 9] = hit[:, 4:, 11] = True
+    assert got[hit].isnan().all() and ((got.double() - want).abs() <= tol)[~hit].all()
