@@ -750,18 +750,19 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
 // of 4 a row has the four warps of a CTA, every fourth piece each: where there are few rows, they have many pieces, and too few warps to have
 // their loads in flight.  (512 rows of 16 requests behind 16384 rows: attention in 29.6 us, by one warp a row 32.9; 2048 rows of 64: 60.4 and
 // 58.0.)
-template <typename T, int HD, int WAYS>
-__global__ void __launch_bounds__(128, 8) paged_join_kernel(const __grid_constant__ PagedParams p, int ctas) {
-    pdl_launch_dependents();
+// True: something of the row is not finite, and it has to be looked at AGAIN, from the start, so that what that needs is not held in registers meanwhile (4 x 1000
+// tokens of 32 heads 271 us, in one loop 302; by a call of a function 277).
+template <typename T, int HD, int WAYS, bool AGAIN>
+__device__ __forceinline__ bool join_row(const PagedParams& p, int ctas) {
     constexpr int N = HD / 32, BATCH = 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = blockIdx.x;
     const int head = WAYS == 1 ? blockIdx.y * 4 + warp : blockIdx.y, way = WAYS == 1 ? 0 : warp;
     // Whose token it is does not depend on the attention, which starts this kernel only once all ahead of it is there: these reads pass while its
     // last CTAs work (64 requests behind 16384 rows 58.2 -> 56.6 us, 4 short ones 11.3 -> 10.7, though 557 -> 566 where the join has 32768 rows).  Who
     // has nothing to do waits all the same: a kernel behind this one must not start ahead of the attention's end.
-    if (head >= p.heads || t < __ldcg(p.row_starts) || t >= __ldcg(p.row_starts + p.requests)) {
+    if (!AGAIN && (head >= p.heads || t < __ldcg(p.row_starts) || t >= __ldcg(p.row_starts + p.requests))) {
         pdl_wait();
-        return;
+        return false;
     }
     int lo = 0, hi = p.requests;
     while (hi - lo > 1) {
@@ -771,7 +772,7 @@ __global__ void __launch_bounds__(128, 8) paged_join_kernel(const __grid_constan
         hi = min(hi, lo + step);
     }
     const Request q = request_of(p, lo);
-    pdl_wait();
+    if (!AGAIN) pdl_wait();
     const Line& l = p.line;
     const int singles = p.plan[p.requests + 1];
     const Share single(l.odd + p.plan[p.requests], 2 * singles);
@@ -826,8 +827,9 @@ __global__ void __launch_bounds__(128, 8) paged_join_kernel(const __grid_constan
     }
     auto count = [](const Segment& s) { return s.from < 0 ? 0 : s.to - s.from + 1; };
     const int n0 = count(seg[0]), n1 = n0 + count(seg[1]), n = n1 + count(seg[2]);
-    // (`again`: without the row's own segment, see below)
-    for (bool again = false;; again = true) {
+    // Again: the own pieces; then, if they are not finite, the others and the own rows one by one, or else all.
+    enum { kOthers = 1, kOwn = 2, kAll = 3 };
+    for (int turn = AGAIN ? kOwn : kAll;;) {
         float m = -INFINITY, sum = 0.f, o[N] = {};
 #pragma unroll 1
         for (int base = 0; base < n; base += 32 * WAYS) {
@@ -835,7 +837,7 @@ __global__ void __launch_bounds__(128, 8) paged_join_kernel(const __grid_constan
             const int k = base + lane * WAYS + way;
             const float* src = nullptr;
             float2 x = make_float2(-INFINITY, 0.f);
-            if (k < n && !(again && k >= n0 && k < n1)) {
+            if (k < n && (k >= n0 && k < n1 ? turn & kOwn : turn & kOthers)) {
                 auto pick = [&](auto a, auto b, auto c) { return k < n0 ? a : (k < n1 ? b : c); };      // (by value: the segments stay in registers)
                 const int j = k - pick(0, n0, n1), w = pick(seg[0].from, seg[1].from, seg[2].from) + j;
                 if (j == 0) {
@@ -884,7 +886,7 @@ __global__ void __launch_bounds__(128, 8) paged_join_kernel(const __grid_constan
         }
         if constexpr (WAYS > 1) {
             __shared__ float s_m[WAYS], s_sum[WAYS], s_o[WAYS][HD];
-            if (again) __syncthreads();
+            if (AGAIN && turn != kOwn) __syncthreads();
             if (lane == 0) {
                 s_m[way] = m;
                 s_sum[way] = sum;
@@ -904,15 +906,21 @@ __global__ void __launch_bounds__(128, 8) paged_join_kernel(const __grid_constan
                 for (int e = 0; e < N; e++) o[e] += a * s_o[w][lane * N + e];
             }
         }
-        if (!again) {
-            // Inf and NaN in the values of new rows that this row does not see have come in as 0 x Inf or NaN.  That is seldom: where anything is not finite, the
-            // row's own rows are gone through one by one, and those that it does not see are left out.
+        // Inf and NaN in the values of new rows that this row does not see have come in as 0 x Inf or NaN.  That is seldom: where anything of its own rows is
+        // not finite, they are gone through one by one, and those that it does not see are left out.  (Not for what the prefix holds, which all see.)
+        if (!AGAIN || turn == kOwn) {
             bool bad = !(fabsf(sum) < INFINITY);
 #pragma unroll
             for (int e = 0; e < N; e++) bad = bad || !(fabsf(o[e]) < INFINITY);
-            if (__any_sync(0xffffffffu, bad)) continue;                      // (of four warps, all)
-        } else {
-            if (way > 0) return;
+            bad = __any_sync(0xffffffffu, bad);                              // (of four warps, all)
+            if (AGAIN) {
+                turn = bad ? kOthers : kAll;
+                continue;
+            }
+            if (bad) return true;
+        }
+        if (AGAIN && turn == kOthers) {
+            if (way > 0) return false;
             const T* mine = static_cast<const T*>(p.q) + t * p.q_token + head * p.q_head + lane * N;
             float x[N];
 #pragma unroll
@@ -937,14 +945,19 @@ __global__ void __launch_bounds__(128, 8) paged_join_kernel(const __grid_constan
                 m = high;
             }
         }
-        if (WAYS > 1 && way > 0) return;
+        if (WAYS > 1 && way > 0) return false;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         Vec<T, N> y;
 #pragma unroll
         for (int e = 0; e < N; e++) y.v[e] = from_f32<T>(o[e] * inv);
         store_vec<true>(static_cast<T*>(p.out) + t * p.out_token + head * p.out_head + lane * N, y, N);
-        return;
+        return false;
     }
+}
+template <typename T, int HD, int WAYS>
+__global__ void __launch_bounds__(128, 8) paged_join_kernel(const __grid_constant__ PagedParams p, int ctas) {
+    pdl_launch_dependents();
+    if (join_row<T, HD, WAYS, false>(p, ctas)) join_row<T, HD, WAYS, true>(p, ctas);
 }
 
 struct Room {
