@@ -1024,7 +1024,7 @@ int b200_paged_attention(const b200_paged* c, const void* q, long long q_token, 
     if ((c->head_dim != 64 && c->head_dim != 128) || !(scale >= 0.f && scale <= 3e38f) || prefix_length < 0 || (prefix_length > 0 && !prefix_pages)) return B200_EINVAL;
     if ((c->page_size < 128 && (c->page_size < 8 || (c->page_size & (c->page_size - 1)))) || (c->page_size > 128 && c->page_size % 128)) return B200_EINVAL;
     constexpr int kMaxRows = 1 << 30;                                   // (rows and what is added to them stay in 32 bits)
-    if (c->requests > kPgMaxRequests || prefix_length > kMaxRows || (long long)c->table_width * c->page_size > kMaxRows) return B200_ELIMIT;
+    if (c->requests > kPgMaxRequests || prefix_length > kMaxRows || c->page_size > kMaxRows || (long long)c->table_width * c->page_size > kMaxRows) return B200_ELIMIT;
     if (c->tokens == 0 || c->requests == 0) return B200_OK;
     if (!q || !out || !workspace || !error) return B200_EINVAL;
     if (workspace_bytes < b200_paged_attention_workspace_bytes(c)) return B200_EWORKSPACE;

@@ -133,3 +133,10 @@ def test_the_error_word_is_found_however_its_device_is_named(be, monkeypatch):
     assert be.paged.attention_error(0, clear=True) == 31 and be.paged.attention_error(0) == 0
     monkeypatch.setattr(be.paged, "_errors", {})
     assert be.paged.attention_error("cuda") == 0
+
+
+def test_a_page_of_more_rows_than_are_counted_is_refused(be):
+    """Also where no table makes more of them."""
+    lib, (buf, base) = be._lib.lib(), _memory()
+    c = _cache(be, base, page_size=(1 << 30) + 128, table_width=0, page_table=None)
+    assert lib.b200_paged_attention(ctypes.byref(c), base, 256, 64, base, 256, 64, base, 5, None, 0.125, base, 1 << 40, base, None) == -6
