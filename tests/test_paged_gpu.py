@@ -8,6 +8,8 @@ probabilities below 2^-14 are off by up to 2^-25 in place of e p, relative to th
 at least 1."""
 import ctypes
 import math
+import pathlib
+import re
 
 import pytest
 import torch
@@ -692,3 +694,24 @@ def test_nan_in_the_prefix_costs_no_walk_over_the_own_rows(be, cuda, prefix, old
     want[:, heads // 2:, 3] = want[:, :heads // 2] = math.nan
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
     assert longer < 4 * usual, (usual, longer)
+
+
+def test_the_documented_calls_run(be, cuda):
+    """The block of the documentation that serves requests over pages, line by line as it stands."""
+    root = pathlib.Path(__file__).resolve().parent.parent
+    blocks = [b for f in sorted(root.glob("*.md")) for b in re.findall(r"```python\n(.*?)```", f.read_text(), re.S)
+              if all(f"be.{name}(" in b for name in ("PagedKVCache", "rope.frequencies", "paged.append", "paged.attention", "verify_tokens"))]
+    assert blocks
+    g = torch.Generator(device=cuda).manual_seed(4)
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)
+    heads, kv, P, n, V = 8, 2, 40, 7, 50
+    rand = lambda *shape: torch.randn(*shape, device=cuda, generator=g).half()
+    for text in blocks:
+        names = dict(be=be, layers=2, pages=16, kv_heads=kv, config=dict(rope_scaling=dict(type="linear", factor=2.0)), i=1, q=rand(n, heads, 128), k=rand(n, kv, 128),
+                     v=rand(n, kv, 128), page_table=ints(3, 4, 5, 6).view(2, 2), lengths=ints(20, 3), row_starts=ints(0, 4, 7), P=P, prefix=ints(7, 8, 9),
+                     x=rand(n, heads, 128), positions=torch.arange(n, device=cuda), draft_tokens=torch.zeros(2, 3, dtype=torch.int32, device=cuda),
+                     target_probs=torch.rand(2, 4, V, device=cuda, generator=g), draft_probs=torch.rand(2, 3, V, device=cuda, generator=g),
+                     uniforms=torch.rand(2, 4, device=cuda, generator=g))
+        exec(text, names)
+        assert names["o"].shape == (n, heads, 128) and names["o"].isfinite().all() and names["x"].shape == (n, heads, 128) and names["tokens"].shape == (2, 4)
+    torch.cuda.synchronize()
