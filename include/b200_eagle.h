@@ -508,7 +508,7 @@ int b200_kv_compact(void* cache, int layers, int Hkv, int cache_rows, int hd, co
 
 /* Rotation by theta = position * scaling * inv_freqs[i]: (a, b) -> magnitude * (a cos - b sin, a sin + b cos) for the pairs (x[i],
  * x[i + rotary_dim / 2]) or, interleaved, (x[2 i], x[2 i + 1]).  Dims from rotary_dim on pass through.  The angle is reduced to a
- * turn in whole numbers: that of the numbers given to within 2^-24 radians up to 2^37 rows, twice that for every doubling beyond. */
+ * turn in whole numbers: that of the numbers given to within 2^-23 radians up to 2^37 rows, twice that for every doubling beyond. */
 typedef struct b200_rotary {
     const void* positions;      /* [tokens] int32, or int64 */
     const float* inv_freqs;     /* [rotary_dim / 2] */
@@ -565,7 +565,8 @@ int b200_paged_attention(const b200_paged* c, const void* q, long long q_token, 
 /* Speculative sampling from given random numbers.  Drafted token i of a request stands while uniforms[i] * q_i(x_i) < p_i(x_i) and all before
  * it do; the token behind the n that stand is drawn by uniforms[drafts] from max(p_n - q_n, 0) (refused) or p_n (all stand): the lowest j whose sum
  * of weights 0..j exceeds uniforms[drafts] times the sum of all, in 64 bits.  Where p_n - q_n leaves nothing it is drawn from p_n, and where that
- * is empty it is token 0.  target: [requests][drafts + 1][vocab] probabilities (need not sum to one); draft: [requests][drafts][vocab], or NULL for
+ * is empty it is token 0.  target: [requests][drafts + 1][vocab] probabilities (rows that do not sum to one are taken as they are: the draw is by
+ * its sum, the test of a draft is not, and tokens are distributed as the target says only where sums are one); draft: [requests][drafts][vocab], or NULL for
  * drafts that were not drawn (q = 1 at the token); draft_lengths: [requests] drafts in use, or NULL for all.  A drafted token outside
  * the vocabulary is refused.  tokens_out: [requests][drafts + 1], the tokens that stand, the drawn one, then -1; accepted: [requests].
  * dtype (both distributions) F16, BF16 or F32; drafts at most 1024, vocab 2^30, requests 65535. */

@@ -2,7 +2,7 @@
 //
 // Drafted token x_i (drawn from q_i) stands while u_i q_i(x_i) < p_i(x_i).  The token behind the last that stands, n of them, is drawn by
 // u_K from max(p_n - q_n, 0) if x_n was refused and from p_n if all stand: the lowest j whose sum of weights 0..j exceeds u_K times the sum
-// of all.  What comes out is then distributed as tokens drawn from p.  Without q the drafts are taken as certain: x_i stands while
+// of all.  What comes out is then distributed as tokens drawn from p, for p and q that sum to one.  Without q the drafts are taken as certain: x_i stands while
 // u_i < p_i(x_i), and p_n without x_n is what a refusal leaves.
 //
 // Products, differences and sums are in 64 bits: u q is exact there, and a border between two tokens lies where exact sums would put it to within

@@ -97,7 +97,7 @@ def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Ten
     """Keys, rotated, and values of a pass into the pages of their requests, and the rotated queries, in one launch.
 
     ``q (tokens, heads, dim)``, ``k`` and ``v (tokens, kv_heads, dim)``: float16 or bfloat16, tokens and heads may be strided (slices of a fused
-    projection); pages ``(pages, kv_heads, page_size, dim)`` in any order of strides.  A token's position is its row behind ``prefix_length``
+    projection), ``k`` and ``v`` alike (keys that went through a norm of their own are copied beside the values, or both made contiguous); pages ``(pages, kv_heads, page_size, dim)`` in any order of strides.  A token's position is its row behind ``prefix_length``
     rows, or ``positions (tokens,)`` says it (a tree of drafted tokens: rows side by side, positions by depth); the rotation is
     ``rope.rotate``'s.  ``q_out`` may be ``q``.  Rows whose page number lies outside the cache, or that the table is too short for, are dropped.
     Two requests that write one page's row in the same pass leave either's."""

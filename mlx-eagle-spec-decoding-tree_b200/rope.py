@@ -104,7 +104,7 @@ def rotate(x: torch.Tensor, positions: torch.Tensor, inv_freqs: torch.Tensor, *,
     """``x (tokens, heads, dim)`` rotated by ``positions (tokens,)`` times ``scaling_factor * inv_freqs``: the pairs ``(x[i], x[i + R/2])``, or
     ``interleaved`` ``(x[2i], x[2i + 1])``, of the first ``R = 2 * len(inv_freqs)`` dims become ``magnitude * (a cos - b sin, a sin + b cos)``; the rest
     passes through.  float16, bfloat16 or float32, fp32 inside, rounded once; tokens and heads may be strided (a slice of a fused
-    projection).  Positions are int32 or int64; an angle is off by less than 2^-24 radians, fp32's own step, up to 2^37 rows, and by twice that a doubling beyond.
+    projection).  Positions are int32 or int64; an angle is off by less than 2^-23 radians up to 2^37 rows, and by twice that a doubling beyond.
 
     ``inverse`` rotates by the negative angle: the gradient of a rotation with respect to ``x`` is the rotation of the result's gradient
     with ``inverse`` and the same magnitude.  ``out`` may be ``x`` itself; other overlaps are undefined.  No gradient is recorded."""

@@ -20,10 +20,11 @@ def verify_tokens(draft_tokens: torch.Tensor, target_probs: torch.Tensor, unifor
     Token ``i`` of ``draft_tokens (B, K)`` int32 stands while ``uniforms[i] * q_i(x_i) < p_i(x_i)`` and those before it do, ``p`` =
     ``target_probs (B, K + 1, V)``, ``q`` = ``draft_probs (B, K, V)`` (None: the drafts were not drawn, ``q`` is 1 at them).  The token behind the ``n`` that
     stand is drawn by ``uniforms[K]`` from ``max(p_n - q_n, 0)``, or from ``p_n`` if all stand: the lowest ``j`` whose sum of weights ``0 .. j`` exceeds
-    ``uniforms[K]`` times the sum of all.  With ``uniforms (B, K + 1)`` float32 independent in [0, 1) the tokens are distributed as drawn from the
-    target.  ``draft_lengths (B,)`` int32 says how many drafts a request has (None: ``K``); the row of ``p`` behind the last of them is used.
+    ``uniforms[K]`` times the sum of all.  With ``uniforms (B, K + 1)`` float32 independent in [0, 1) and rows that sum to one the tokens are distributed as
+    drawn from the target.  ``draft_lengths (B,)`` int32 says how many drafts a request has (None: ``K``); the row of ``p`` behind the last of them is used.
 
-    Distributions are float32, float16 or bfloat16, both of one type, any strides but a contiguous last dimension; they need not sum to one.
+    Distributions are float32, float16 or bfloat16, both of one type, any strides but a contiguous last dimension.  Rows of another sum
+    are taken as they are: the draw goes by its weights' sum, whether a draft stands does not.
     Products, differences and sums are in 64 bits.  A drafted token outside the vocabulary is refused; where ``p_n - q_n`` leaves nothing, the
     token is drawn from ``p_n``, and where that is empty it is 0.  ``K`` at most 1024."""
     both = _lib.ops().verify_tokens(draft_tokens, target_probs, uniforms, draft_probs, draft_lengths)
