@@ -555,8 +555,8 @@ int b200_paged_append(const b200_paged* c, const b200_rotary* r, const void* q, 
  * outside the cache stands for rows of zeros.  out may be q with the same strides.  scale is finite and 0 or more.  head_dim 64 or 128; page_size 8,
  * 16, 32, 64 or a multiple of 128; strides positive multiples of 8, pointers 16-byte aligned; at most 1024 requests, 2^30 rows of a
  * page, of a prefix or of a row of the table.
- * workspace: b200_paged_attention_workspace_bytes(c) bytes, 16-byte aligned, of any content, not shared with a call that may run at the same
- * time.  error: device word, zero at first; not zero after a wait inside the kernel that ran out. */
+ * workspace: b200_paged_attention_workspace_bytes(c) bytes (12 for each value of the result, and 39 MB for heads of 128, 20 MB for heads of 64), 16-byte
+ * aligned, of any content, not shared with a call that may run at the same time.  error: device word, zero at first; not zero after a wait inside the kernel that ran out. */
 size_t b200_paged_attention_workspace_bytes(const b200_paged* c);
 int b200_paged_attention(const b200_paged* c, const void* q, long long q_token, long long q_head, void* out, long long out_token, long long out_head,
                          const int* prefix_pages, int prefix_length, const unsigned long long* mask, float scale, void* workspace,

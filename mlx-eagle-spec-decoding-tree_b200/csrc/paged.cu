@@ -18,7 +18,7 @@
 // Every wait is bounded; one that runs out sets the error word and goes on.  No copy uses cluster multicast.
 //
 // What bounds it: for pairs the chain of products, softmax and waits (4240 cycles a block of 256 rows, 2144 of them products: 16 x 64 tokens of 32
-// heads behind 32768 rows 505 us, 1.1 PFLOP/s, and 580 at the power limit); for single streams the copies (64 x 1 tokens behind 16384 rows, 1024 rows
+// heads behind 32768 rows 505 us, 1.1 PFLOP/s, and 576 at the power limit); for single streams the copies (64 x 1 tokens behind 16384 rows, 1024 rows
 // each: 65 us, 3.2 TB/s), and where they are short the start and the join, some 10 us.
 #include <algorithm>
 #include <atomic>
@@ -748,8 +748,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_kernel(const __grid_const
 
 // A warp joins the pieces of one query row: a lane looks at a piece's statistics, then all lanes add its output, four dims (two) each.  With WAYS
 // of 4 a row has the four warps of a CTA, every fourth piece each: where there are few rows, they have many pieces, and too few warps to have
-// their loads in flight.  (512 rows of 16 requests behind 16384 rows: attention in 29.6 us, by one warp a row 32.9; 2048 rows of 64: 60.4 and
-// 58.0.)
+// their loads in flight.  (512 rows of 16 requests behind 16384 rows: attention in 34.7 us, by one warp a row 38.2; 2048 rows of 64: 86 and
+// 81; the two meet at some 1300.)
 // True: something of the row is not finite, and it has to be looked at AGAIN, from the start, so that what that needs is not held in registers meanwhile (4 x 1000
 // tokens of 32 heads 271 us, in one loop 302; by a call of a function 277).
 template <typename T, int HD, int WAYS, bool AGAIN>
@@ -758,7 +758,7 @@ __device__ __forceinline__ bool join_row(const PagedParams& p, int ctas) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = blockIdx.x;
     const int head = WAYS == 1 ? blockIdx.y * 4 + warp : blockIdx.y, way = WAYS == 1 ? 0 : warp;
     // Whose token it is does not depend on the attention, which starts this kernel only once all ahead of it is there: these reads pass while its
-    // last CTAs work (64 requests behind 16384 rows 58.2 -> 56.6 us, 4 short ones 11.3 -> 10.7, though 557 -> 566 where the join has 32768 rows).  Who
+    // last CTAs work (64 requests behind 16384 rows 58.2 -> 56.6 us, 4 short ones 11.3 -> 10.7, though 557 -> 566 where the join has 32768 rows: measured when this was moved).  Who
     // has nothing to do waits all the same: a kernel behind this one must not start ahead of the attention's end.
     if (!AGAIN && (head >= p.heads || t < __ldcg(p.row_starts) || t >= __ldcg(p.row_starts + p.requests))) {
         pdl_wait();

@@ -24,15 +24,15 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// Bounded wait: false if the phase did not complete within `polls`.  A poll that does not find the phase complete suspends the thread for up to about a
-// microsecond, so the limit is a time limit.  (Without a suspend-time hint a complete phase is seen in 14 cycles and a
+// Bounded wait: false if the phase did not complete within `polls`.  A poll that does not find the phase complete suspends the thread for up to 7758
+// cycles (4 us), so the limit is a time limit.  (Without a suspend-time hint a complete phase is seen in 14 cycles and a
 // suspended thread is back ~60 cycles after the arrival; with a hint the same two took 100 and 75 to 100 cycles.)
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t polls) {
     for (uint32_t i = 0; i < polls; i++)
         if (mbar_try_wait(bar, parity)) return true;
     return false;
 }
-constexpr int kWaitPolls = 1 << 19;             // of a wait before it reports: half a second
+constexpr int kWaitPolls = 1 << 19;             // of a wait before it reports: two seconds
 constexpr int kFirmPolls = 8 * kWaitPolls;      // after which it is over all the same
 constexpr int kNoReport = kFirmPolls;
 // A wait that runs out of its polls sets the error word (kNoReport: there is none) and goes on, for some seconds in all: what it waits for

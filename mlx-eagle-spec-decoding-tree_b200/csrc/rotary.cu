@@ -10,7 +10,7 @@
 // 2^31 and 1.2e-4 at 2^40).  Products and sums of a pair are fp32, rounded once to the result's type.
 //
 // A CTA has a token or two: its threads turn the angles once (the only costly arithmetic), then all go over the heads, 16 bytes an item, two in
-// flight.  What bounds it: instructions (address, conversion) and the wait for the angles; 4099 tokens of 32 x 128 16-bit elements 13.3 us (5.0 TB/s, 77 %
+// flight.  What bounds it: the wait for loads and angles, a third of an SM's warps being there to pass it (80 registers), and instructions; 4099 tokens of 32 x 128 16-bit elements 13.3 us (5.0 TB/s, 77 %
 // of a copy's rate; 13.2 with the fraction from one double), ragged prompts 49.4 (4.3 TB/s, 65 %; 49.3), one token 3.9 (the launch).
 #include <algorithm>
 #include <cmath>

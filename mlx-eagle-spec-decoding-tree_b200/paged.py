@@ -97,9 +97,10 @@ def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Ten
     """Keys, rotated, and values of a pass into the pages of their requests, and the rotated queries, in one launch.
 
     ``q (tokens, heads, dim)``, ``k`` and ``v (tokens, kv_heads, dim)``: float16 or bfloat16, tokens and heads may be strided (slices of a fused
-    projection), ``k`` and ``v`` alike (keys that went through a norm of their own are copied beside the values, or both made contiguous); pages ``(pages, kv_heads, page_size, dim)`` in any order of strides.  A token's position is its row behind ``prefix_length``
-    rows, or ``positions (tokens,)`` says it (a tree of drafted tokens: rows side by side, positions by depth); the rotation is
-    ``rope.rotate``'s.  ``q_out`` may be ``q``.  Rows whose page number lies outside the cache, or that the table is too short for, are dropped.
+    projection), ``k`` and ``v`` alike (where a norm has made new keys, values are made contiguous too); pages ``(pages, kv_heads, page_size, dim)`` in any
+    order of strides.  A token's position is its row behind ``prefix_length`` rows, or ``positions (tokens,)`` says it (a tree of drafted tokens: rows
+    side by side, positions by depth); the rotation is ``rope.rotate``'s.  ``q_out`` may be ``q``.  Rows whose page number lies outside the cache, or that
+    the table is too short for, are dropped.
     Two requests that write one page's row in the same pass leave either's."""
     if q_out is None:
         y = _lib.ops().paged_append(q, k, v, k_pages, v_pages, page_table, lengths, row_starts, prefix_length, positions, inv_freqs, scaling_factor,
@@ -149,7 +150,9 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     ``q (tokens, heads, dim)``, positions already in it; heads of 64 or 128; float16 or bfloat16, scores, statistics and sums in fp32, probabilities
     rounded to the type for the second product; NaN and infinities reach the tokens that see them, and no other.  ``out`` may be ``q``.  ``scale``, 0 or more, is
     ``dim ** -0.5`` unless given.  A token that sees no row gets zeros; results of tokens outside ``row_starts`` are
-    not written (``append`` likewise).  Rows behind a length may hold anything; a page number outside the cache stands for rows of zeros.  At most 1024 requests."""
+    not written (``append`` likewise).  Rows behind a length may hold anything; a page number outside the cache stands for rows of zeros.  At most 1024 requests.
+    Rows of ``q``, ``out`` and the pages start at 16 bytes (strides of multiples of 8).  A call takes a workspace of 12 bytes for each value of the result and 39 MB (heads of
+    128; 20 MB of 64); the prefix is gone over for all ``tokens``, padding among them."""
     if out is None and isinstance(q, torch.Tensor):
         y = _lib.ops().paged_attention(q, k_pages, v_pages, page_table, lengths, row_starts, prefix_pages, prefix_length, mask, scale,
                                        _errors.get(q.device.index))
